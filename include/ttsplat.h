@@ -55,6 +55,9 @@ extern "C" {
 #define TTS_ERADIUS (-7)    /* stencil radius other than 1 */
 #define TTS_ESH (-8)        /* SH degree outside [0, 3], or rest coefficients missing */
 #define TTS_ESCRATCH (-9)   /* sizes beyond the fixed scratch of an allocation-free entry point */
+#define TTS_EDTYPE (-10)    /* element type not TTS_F32/F16/BF16, or weights of a third type */
+#define TTS_ELENGTH (-11)   /* a length over an entry's limit */
+#define TTS_EHEADS (-12)    /* head size outside [1, 128], or heads not a multiple of kv_heads */
 
 /* Library version, (major << 16) | minor. */
 int tts_version(void);
@@ -607,6 +610,45 @@ int tts_wsr_dense_bwd(const float* theta, const float* o, const float* color,
                       const uint8_t* keep, const float* phi, int G, int P, const float* bg,
                       const float* C, const float* den, const float* gC, float* gtheta10,
                       float* gwb, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---- operators of token networks beside a scene (codes of gaussians and of a view's tokens);
+ * the reference has no counterpart ---- */
+
+/* Element types.  Sums, statistics and softmax are held in 32 bits; results are rounded once. */
+#define TTS_F32 0
+#define TTS_F16 1
+#define TTS_BF16 2
+
+/* Layer norm of x [rows, cols] (rows x_stride elements apart, cols contiguous, any alignment of
+ * the element): y [rows, cols] contiguous = (x - mean) / sqrt(var + eps) * weight + bias, var the mean
+ * of squared deviations.  weight, bias [cols] of x's type or fp32 (w_dtype; both the same type),
+ * NULL for 1 and 0.  stats [rows][2] = (mean, 1 / sqrt(var + eps)), NULL where no backward follows. */
+int tts_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias,
+                       int64_t rows, int cols, float eps, int dtype, int w_dtype, void* y,
+                       float* stats, hipStream_t stream);
+
+size_t tts_layer_norm_workspace_bytes(int64_t rows, int cols, int dtype);
+
+/* Its backward from stats: dx [rows, cols] contiguous, dweight, dbias [cols] of w_dtype; each may be
+ * NULL (not all).  Deterministic: the rows' sums run in a fixed order.  The workspace is needed for
+ * dweight and dbias only. */
+int tts_layer_norm_bwd(const void* x, int64_t x_stride, const void* weight, const void* dy,
+                       int64_t dy_stride, const float* stats, int64_t rows, int cols, int dtype,
+                       int w_dtype, void* dx, void* dweight, void* dbias, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+/* Embedding lookup: out[t] = scale * table[ids[t]], table [V, D], ids int32 or int64 (ids64); an id
+ * outside [0, V) gives a row of zeros.  V, N up to 2^30. */
+int tts_embedding_fwd(const void* table, int64_t V, int D, const void* ids, int ids64, int64_t N,
+                      float scale, int dtype, void* out, hipStream_t stream);
+
+size_t tts_embedding_workspace_bytes(int64_t N, int64_t V, int D);
+
+/* Its gradient: dtable[v] = scale * sum of dout[t] over the tokens of id v, every row written.
+ * Deterministic: the tokens are sorted by id and summed in a fixed order. */
+int tts_embedding_bwd(const void* dout, const void* ids, int ids64, int64_t N, int64_t V, int D,
+                      float scale, int dtype, void* dtable, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

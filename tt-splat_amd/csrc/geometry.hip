@@ -1367,6 +1367,9 @@ const char* tts_strerror(int code) {
     case TTS_EG: return "G must be below 2^30 (at most 2^28 for binning)";
     case TTS_ERADIUS: return "only stencil radius R = 1 is supported";
     case TTS_ESH: return "SH degree must be in [0, 3], with rest coefficients when above 0";
+    case TTS_EDTYPE: return "element type must be fp32, fp16 or bf16 (weights: the rows' type or fp32)";
+    case TTS_ELENGTH: return "length over the limit (embedding: 2^30 ids and rows; attention: 2^30 rows or keys)";
+    case TTS_EHEADS: return "head size must be in [1, 128] and query heads a multiple of key heads";
     case TTS_ESCRATCH: return "sizes exceed the fixed scratch of the allocation-free entry point";
     default: return code > 0 ? hipGetErrorString(static_cast<hipError_t>(code)) : "unknown error";
   }

@@ -129,6 +129,16 @@ SIGNATURES = {
     "tts_wsr_dense": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "tts_wsr_dense_bwd": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _vp, _vp, _vp, _vp,
                                    _vp, _vp, _vp, _c_size, _vp]),
+    "tts_layer_norm_fwd": (_c_int, [_vp, _c_i64, _vp, _vp, _c_i64, _c_int, _c_float, _c_int,
+                                    _c_int, _vp, _vp, _vp]),
+    "tts_layer_norm_workspace_bytes": (_c_size, [_c_i64, _c_int, _c_int]),
+    "tts_layer_norm_bwd": (_c_int, [_vp, _c_i64, _vp, _vp, _c_i64, _vp, _c_i64, _c_int, _c_int,
+                                    _c_int, _vp, _vp, _vp, _vp, _c_size, _vp]),
+    "tts_embedding_fwd": (_c_int, [_vp, _c_i64, _c_int, _vp, _c_int, _c_i64, _c_float, _c_int,
+                                   _vp, _vp]),
+    "tts_embedding_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_int]),
+    "tts_embedding_bwd": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_i64, _c_int, _c_float, _c_int,
+                                   _vp, _vp, _c_size, _vp]),
 }
 
 _lib = None

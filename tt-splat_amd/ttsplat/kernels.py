@@ -1019,3 +1019,135 @@ def wsr_dense_bwd(theta, o, color, keep, phi, bg, C, den, gC, workspace=None):
          ptr(bg), ptr(C), ptr(den), ptr(gC), ptr(g10), ptr(gwb), ptr(workspace),
          workspace.numel(), stream())
     return g10[:, 0:6], g10[:, 6], g10[:, 7:10], gwb
+
+
+# ------------------------------------------------------------- token networks beside a scene --
+DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _elem(t, name, device=None, dtype=None):
+    """Type code of a GPU tensor of fp32, fp16 or bf16 (of `dtype`, on `device`)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor (got {t.device}); the HIP path has no CPU fallback")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    code = DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _norm_rows(x, name, device=None, dtype=None, shape=None):
+    code = _elem(x, name, device, dtype)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"{name} must be [rows, cols] with cols >= 1, got {tuple(x.shape)}")
+    if shape is not None and x.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(x.shape)}, expected {tuple(shape)}")
+    if x.shape[1] > 1 and x.stride(1) != 1:
+        raise ValueError(f"{name} must have contiguous columns")
+    return code
+
+
+def _norm_weights(x, weight, bias):
+    """Type code of the weights: x's type or fp32, one type for both."""
+    code = None
+    for t, n in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        c = _elem(t, n, x.device)
+        if t.shape != (x.shape[1],) or not t.is_contiguous():
+            raise ValueError(f"{n} must be contiguous [{x.shape[1]}], got {tuple(t.shape)}")
+        if t.dtype != x.dtype and t.dtype != F32:
+            raise ValueError(f"{n} must be {x.dtype} or float32, got {t.dtype}")
+        if code is not None and c != code:
+            raise ValueError("weight and bias must have the same type")
+        code = c
+    return 0 if code is None else code
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, y=None, stats=None):
+    """y [rows, cols] = layer norm of x's rows (columns contiguous, any row stride); stats
+    [rows, 2] fp32, when given, takes each row's (mean, 1/sqrt(var + eps))."""
+    code = _norm_rows(x, "x")
+    wcode = _norm_weights(x, weight, bias)
+    R, D = x.shape
+    y = torch.empty(R, D, device=x.device, dtype=x.dtype) if y is None else y
+    require(y, "y", x.dtype, (R, D), x.device)
+    if stats is not None:
+        require(stats, "stats", F32, (R, 2), x.device)
+    call("tts_layer_norm_fwd", ptr(x), x.stride(0), ptr(weight), ptr(bias), R, D, float(eps), code,
+         wcode, ptr(y), ptr(stats), stream())
+    return y
+
+
+def layer_norm_bwd(x, weight, dy, stats, dx=True, dweight=True, dbias=True, w_dtype=None):
+    """(dx, dweight, dbias) from the forward's stats; a False argument leaves that result out
+    (None).  dweight and dbias are of weight's type (w_dtype where there is no weight)."""
+    code = _norm_rows(x, "x")
+    R, D = x.shape
+    dev = x.device
+    _norm_rows(dy, "dy", dev, x.dtype, x.shape)
+    wcode = _norm_weights(x, weight, None)
+    wt = weight.dtype if weight is not None else (w_dtype or x.dtype)
+    if wt != x.dtype and wt != F32:
+        raise ValueError(f"w_dtype must be {x.dtype} or float32, got {wt}")
+    wcode = DTYPE_CODES[wt]
+    require(stats, "stats", F32, (R, 2), dev)
+    gx = torch.empty(R, D, device=dev, dtype=x.dtype) if dx else None
+    gw = torch.empty(D, device=dev, dtype=wt) if dweight else None
+    gb = torch.empty(D, device=dev, dtype=wt) if dbias else None
+    if not (dx or dweight or dbias):
+        return gx, gw, gb
+    ws, n = None, 0
+    if dweight or dbias:
+        n = _lib.load().tts_layer_norm_workspace_bytes(R, D, code)
+        ws = torch.empty(n, device=dev, dtype=U8)
+    call("tts_layer_norm_bwd", ptr(x), x.stride(0), ptr(weight), ptr(dy), dy.stride(0), ptr(stats),
+         R, D, code, wcode, ptr(gx), ptr(gw), ptr(gb), ptr(ws), n, stream())
+    return gx, gw, gb
+
+
+def _ids(ids, device):
+    if not isinstance(ids, torch.Tensor) or ids.dtype not in (I32, torch.int64):
+        raise ValueError("ids must be an int32 or int64 tensor")
+    require(ids, "ids", ids.dtype, None, device)
+    return 1 if ids.dtype == torch.int64 else 0
+
+
+def embedding_fwd(table, ids, scale=1.0, out=None):
+    """out [*ids.shape, D] = scale * table[ids]; ids outside [0, V) give rows of zeros."""
+    code = _elem(table, "table")
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError(f"table must be [V, D], got {tuple(table.shape)}")
+    require(table, "table", table.dtype)
+    V, D = table.shape
+    wide = _ids(ids, table.device)
+    shape = (*ids.shape, D)
+    out = torch.empty(shape, device=table.device, dtype=table.dtype) if out is None else out
+    require(out, "out", table.dtype, shape, table.device)
+    call("tts_embedding_fwd", ptr(table), V, D, ptr(ids), wide, ids.numel(), float(scale), code,
+         ptr(out), stream())
+    return out
+
+
+def embedding_bwd(dout, ids, V, scale=1.0, out=None, workspace=None):
+    """dtable [V, D] = scale * the sum of dout's rows by id (fixed order, every row written)."""
+    code = _elem(dout, "dout")
+    wide = _ids(ids, dout.device)
+    if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape) or dout.shape[-1] < 1:
+        raise ValueError(f"dout must be [*ids.shape, D], got {tuple(dout.shape)}")
+    require(dout, "dout", dout.dtype)
+    D, N = dout.shape[-1], ids.numel()
+    out = torch.empty(V, D, device=dout.device, dtype=dout.dtype) if out is None else out
+    require(out, "out", dout.dtype, (V, D), dout.device)
+    if workspace is None:
+        n = _lib.load().tts_embedding_workspace_bytes(N, V, D)
+        workspace = torch.empty(n, device=dout.device, dtype=U8)
+    require(workspace, "workspace", U8, None, dout.device)
+    call("tts_embedding_bwd", ptr(dout), ptr(ids), wide, N, V, D, float(scale), code, ptr(out),
+         ptr(workspace), workspace.numel(), stream())
+    return out

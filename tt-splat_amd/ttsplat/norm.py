@@ -1,0 +1,51 @@
+"""Layer norm of feature rows on the GPU (no counterpart in the reference).
+
+`layer_norm(x, weight, bias, eps)` is differentiable w.r.t. x, weight and bias.  Rows may be
+fp32, fp16 or bf16, weights of the same type or fp32; statistics and sums are fp32, and the
+gradients of weight and bias are summed over the rows in a fixed order.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import kernels
+
+F32 = torch.float32
+
+
+def _rows(x):
+    """x [..., D] as [rows, D] with contiguous columns (a view wherever one exists)."""
+    D = x.shape[-1]
+    r = x if x.dim() == 2 else x.reshape(-1, D)
+    return r if D == 1 or r.stride(1) == 1 else r.contiguous()
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        rows = _rows(x)
+        stats = torch.empty(rows.shape[0], 2, device=x.device, dtype=F32)
+        y = kernels.layer_norm_fwd(rows, weight, bias, eps, stats=stats)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y.view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        nx, nw, nb, _ = ctx.needs_input_grad
+        dx, dw, db = kernels.layer_norm_bwd(_rows(x), weight, _rows(dy), stats, nx, nw, nb,
+                                            ctx.bias_dtype)
+        return (None if dx is None else dx.view(x.shape)), dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [..., D]."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must be a tensor [..., D] with D >= 1")
+    if torch.is_grad_enabled() and (x.requires_grad
+                                    or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    y = kernels.layer_norm_fwd(_rows(x), weight, bias, eps)
+    return y if x.dim() == 2 else y.view(x.shape)
