@@ -650,6 +650,37 @@ int tts_embedding_bwd(const void* dout, const void* ids, int ids64, int64_t N, i
                       float scale, int dtype, void* dtable, void* workspace,
                       size_t workspace_bytes, hipStream_t stream);
 
+/* Shape of an attention call.  Strides are in elements, of (batch, head, row); the head_dim values of a
+ * row are contiguous; any alignment of the element.  heads is a multiple of kv_heads: query head h
+ * reads key head h / (heads / kv_heads).  The strides o are of out; dout, dq, dk and dv are read by the
+ * backward alone. */
+typedef struct tts_attention_shape {
+  int64_t batch, heads, kv_heads, queries, keys, head_dim;
+  int64_t causal;       /* row i sees keys up to i + keys - queries */
+  int64_t dtype;        /* TTS_F32, TTS_F16 or TTS_BF16, of every tensor */
+  int64_t mask_stride;  /* bytes between the batches of key_mask */
+  int64_t q[3], k[3], v[3], o[3], dout[3], dq[3], dk[3], dv[3];
+  double scale;         /* positive; scores are scale * q . k */
+} tts_attention_shape;
+
+/* Workspace of the forward (0 unless the keys are split) or the backward. */
+size_t tts_attention_workspace_bytes(const tts_attention_shape* shape, int backward);
+
+/* out = softmax(scale q k^T over the visible keys) v.  key_mask (may be NULL): one byte for each batch
+ * and key, 0 hides the key, whose k and v rows may hold anything.  A row that sees no key gives zeros.
+ * lse [batch, heads, queries] fp32 contiguous (may be NULL where no backward follows): the
+ * log-sum-exp of each row's scores, -inf for a row without a key. */
+int tts_attention_fwd(const tts_attention_shape* shape, const void* q, const void* k,
+                      const void* v, const uint8_t* key_mask, void* out, float* lse,
+                      void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Its gradients, from out and lse (the probabilities are recomputed): dq, dk, dv, each may be NULL (not
+ * all).  Hidden keys get zeros.  Deterministic: no atomics.  Sizes of zero are refused. */
+int tts_attention_bwd(const tts_attention_shape* shape, const void* q, const void* k,
+                      const void* v, const uint8_t* key_mask, const void* out, const float* lse,
+                      const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

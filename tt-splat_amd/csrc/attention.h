@@ -1,0 +1,345 @@
+// Attention: what its kernels share (attention_fwd.hip, attention_dq.hip, attention_dkv.hip).
+//
+//   S = c Q K^T (masked places -inf),  L = log sum exp S,  P = exp(S - L),  O = P V
+//   dV = P^T dO,  dP = dO V^T,  D = rowsum(dO O),  dS = P (dP - D),  dQ = c dS K,  dK = c dS^T Q
+//
+// Matrix instructions.  All products run on 32x32 results, 16 deep (eight values a lane and operand):
+//   A (rows of the result): lane l holds row l % 32, places 8 (l / 32) .. + 7 of the depth
+//   B (columns):            lane l holds column l % 32, the same places
+//   result:                 lane l holds column l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4, i = 0..15
+// The order of places along the depth is free as long as A and B agree.  A result's values 8 c ..
+// 8 c + 7 are rows 16 c + 8 (j / 4) + 4 (l / 32) + j % 4 of its column, so they are at once the B
+// operand of a product whose depth is those rows: probabilities go from one product to the next
+// without leaving their lane.  The A operand of that product is a transposed read of a row-major tile
+// in that order (transpose_frag).  Hence each kernel computes the transposes whose column is what the
+// wave owns: S^T and O^T, dQ^T with a query row a column; S, dV^T and dK^T with a key a column.  Row
+// maxima and sums are then sums over a lane's own values and its partner's in the other half.
+//
+// Half types take one 16-deep instruction; fp32 takes eight 2-deep ones over the same registers.
+//
+// Rows.  The query heads that share a key head are rows of one matrix: row r of (batch, key head) is
+// position r / grp of query head kvhead * grp + r % grp, so shared heads cost no second read of K
+// and V, a single token's heads fill a tile together, and dK, dV sum over the group without atomics.
+#pragma once
+
+#include "elem.h"
+#include "lds_limit.h"
+
+namespace tts {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <typename T>
+using Frag = T __attribute__((ext_vector_type(8)));
+using Acc = float __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ Acc mma(Frag<bf16> a, Frag<bf16> b, Acc c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ Acc mma(Frag<f16> a, Frag<f16> b, Acc c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ Acc mma(Frag<float> a, Frag<float> b, Acc c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+
+// Strides in elements of (batch, head, row).
+struct AttnStride {
+  int64_t b, h, n;
+};
+
+struct AttnArgs {
+  const void *q, *k, *v, *o, *dout;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta, *part, *part2;
+  const uint8_t* mask;
+  int64_t mask_stride;
+  AttnStride sq, sk, sv, so, sdo, sdq, sdk, sdv;
+  int Hkv, grp, Nq, Nk, D, R;   // R = Nq * grp rows a (batch, key head)
+  int causal, off;              // row at position p sees keys up to p + off
+  int nsplit;                   // parts of the long axis, joined by a second kernel
+  float scale;
+};
+
+// Position and head of a row.
+__device__ __forceinline__ void attn_row(const AttnArgs& a, int r, int* pos, int* h) {
+  if (a.grp == 1) {
+    *pos = r;
+    *h = 0;
+  } else {
+    *pos = (int)((unsigned)r / (unsigned)a.grp);
+    *h = r - *pos * a.grp;
+  }
+}
+__device__ __forceinline__ int64_t row_offset(const AttnStride& s, int pos, int h) {
+  return h * s.h + pos * s.n;
+}
+
+// Eight values at p, n of them within the row, zeros behind.
+template <typename T>
+__device__ __forceinline__ Frag<T> load_frag(const T* p, int n) {
+  Frag<T> f;
+  if (n >= 8) {
+    memcpy(&f, p, 8 * sizeof(T));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = i < n ? p[i] : (T)0.0f;
+  }
+  return f;
+}
+
+// Tiles in LDS: row-major, rows 16 bytes longer than their data, which spreads the rows of one
+// fragment (32 lanes, 16 bytes each) and of one transposed read over the banks.
+template <typename T, int DP>
+constexpr int kTileStride = DP + 16 / (int)sizeof(T);
+
+template <typename T, int DP>
+__device__ __forceinline__ Frag<T> tile_frag(const T* tile, int row0, int d0) {
+  const int lane = threadIdx.x & 63;
+  Frag<T> f;
+  memcpy(&f, __builtin_assume_aligned(tile + (row0 + (lane & 31)) * kTileStride<T, DP> + d0 +
+                                          (lane >> 5) * 8, 16), 8 * sizeof(T));
+  return f;
+}
+
+// A operand whose rows are the tile's columns d0 .. d0 + 31 and whose depth is its rows row0 ..
+// row0 + 15, in the order of a result's values: place j is row 8 (j / 4) + 4 (lane / 32) + j % 4.
+template <typename T, int DP>
+__device__ __forceinline__ Frag<T> transpose_frag(const T* tile, int row0, int d0) {
+  const int lane = threadIdx.x & 63, hi = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    // ds_read_tr16_b64: 16 lanes read a 4 x 16 block (lane l: row l / 4, columns 4 (l % 4) ..) and
+    // lane l receives column l
+    using S4 = short __attribute__((ext_vector_type(4)));
+    using LdsPtr = __attribute__((address_space(3))) S4*;
+    const T* p = tile + (row0 + 4 * hi + ((lane & 15) >> 2)) * kTileStride<T, DP> + d0 +
+                 (lane & 16) + 4 * (lane & 3);
+    const S4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)p);
+    const S4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + 8 * kTileStride<T, DP>));
+    const short __attribute__((ext_vector_type(8))) r =
+        __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(Frag<T>, r);
+  } else {
+    Frag<T> f;
+    const T* p = tile + (row0 + 4 * hi) * kTileStride<T, DP> + d0 + (lane & 31);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = p[(8 * (j >> 2) + (j & 3)) * kTileStride<T, DP>];
+    return f;
+  }
+}
+
+// One tile of BN rows on its way from memory to LDS through registers: load() starts the reads, store()
+// writes the tile, zeros for rows not in `live` (masked and missing keys: whatever stands there, NaN
+// among it, stays out of the products) and past the head size.
+template <typename T, int DP, int BN, int NT>
+struct TileLoad {
+  static constexpr int kPerRow = DP / 8, kN = BN * kPerRow / NT;
+  static_assert(kN * NT == BN * kPerRow, "threads must divide the tile");
+  Frag<T> r[kN];
+
+  // row(i): offset of the tile's row i (any valid row for rows that are not live)
+  template <typename Row>
+  __device__ __forceinline__ void load(const T* base, int D, Row row) {
+    if ((D & 7) == 0) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int v = threadIdx.x + i * NT, d0 = v % kPerRow * 8;
+        memcpy(&r[i], base + row(v / kPerRow) + (d0 < D ? d0 : 0), 8 * sizeof(T));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int v = threadIdx.x + i * NT, d0 = v % kPerRow * 8;
+        r[i] = load_frag(base + row(v / kPerRow) + d0, D - d0);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* tile, uint64_t live, int D) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int v = threadIdx.x + i * NT, n = v / kPerRow, d0 = v % kPerRow * 8;
+      const bool on = ((live >> n) & 1) && d0 < D;
+      Frag<T> f = r[i];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = on ? f[j] : (T)0.0f;
+      memcpy(__builtin_assume_aligned(tile + n * kTileStride<T, DP> + d0, 16), &f, 8 * sizeof(T));
+    }
+  }
+};
+
+// Non-zero bytes of x as four bits.
+__device__ __forceinline__ uint32_t byte_bits(uint32_t x) {
+  const uint32_t y = ((((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x) & 0x80808080u) >> 7;
+  return (y * 0x10204080u) >> 28;
+}
+
+// Live keys of the tile at key k0 (BN of them), as bits.
+template <int BN>
+__device__ __forceinline__ uint64_t live_keys(const uint8_t* mask, int k0, int Nk) {
+  const int n = Nk - k0;
+  if (n <= 0) return 0;
+  const uint64_t all = n >= BN ? (BN == 64 ? ~0ull : (1ull << BN) - 1) : (1ull << n) - 1;
+  if (!mask) return all;
+  uint64_t w = 0;
+  if (n >= BN) {
+#pragma unroll
+    for (int i = 0; i < BN / 16; ++i) {
+      uint32_t x[4];
+      memcpy(x, mask + k0 + 16 * i, 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w |= (uint64_t)byte_bits(x[j]) << (16 * i + 4 * j);
+    }
+  } else {
+    for (int i = 0; i < n; ++i) w |= (uint64_t)(mask[k0 + i] != 0) << i;
+  }
+  return w;
+}
+
+// Tiles [t, end) that hold a live key, 64 tiles at a time: lane i holds the bits of tile base + i.
+// The same in every wave of a block.
+template <int BN>
+struct KeyTiles {
+  const uint8_t* mask;
+  int Nk, base, end;
+  uint64_t word, pending;
+
+  __device__ __forceinline__ void start(const uint8_t* m, int nk, int t, int t_end) {
+    mask = m;
+    Nk = nk;
+    base = t;
+    end = t_end;
+    fill();
+  }
+  __device__ __forceinline__ void fill() {
+    const int t = base + (int)(threadIdx.x & 63);
+    word = t < end ? live_keys<BN>(mask, t * BN, Nk) : 0;
+    pending = __ballot(word != 0);
+  }
+  __device__ __forceinline__ bool next(int* tile, uint64_t* live) {
+    while (!pending) {
+      if (base + 64 >= end) return false;
+      base += 64;
+      fill();
+    }
+    const int b = __builtin_ctzll(pending);
+    pending &= pending - 1;
+    *tile = base + b;
+    *live = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)word, b) |
+            (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(word >> 32), b) << 32;
+    return true;
+  }
+};
+
+__device__ __forceinline__ float max_halves(float x) {
+  const float2 s = swap_halves(x);
+  return fmaxf(s.x, s.y);
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const float2 s = swap_halves(x);
+  return s.x + s.y;
+}
+
+// Each row's dot product of x and y (fragments of the same 32 rows), in both halves: the diagonal of
+// x y^T.  Its terms are added in the order of every product here, so that for a row with one visible
+// key, where O = V, rowsum(dO O) equals dO V^T to the last bit and dS is zero.
+template <typename T, int KC>
+__device__ __forceinline__ float row_dots(const Frag<T> (&x)[KC], const Frag<T> (&y)[KC]) {
+  const int col = threadIdx.x & 31, hi = (threadIdx.x & 63) >> 5;
+  Acc s = {};
+#pragma unroll
+  for (int c = 0; c < KC; ++c) s = mma(x[c], y[c], s);
+  float r = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r = 8 * (i >> 2) + 4 * hi + (i & 3) == col ? s[i] : r;
+  const float2 w = swap_halves(r);
+  return (col >> 2) & 1 ? w.y : w.x;
+}
+
+// exp2 by the hardware instruction: exp2(-inf) = 0, one unit in the last place.
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Eight of a result's values as an operand, rounded to the operands' type.
+template <typename T>
+__device__ __forceinline__ Frag<T> acc_frag(const Acc& s, int c) {
+  Frag<T> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (T)s[8 * c + j];
+  return f;
+}
+
+// Four consecutive values of a row, n of them within it.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int n, float x0, float x1, float x2, float x3) {
+  const T v[4] = {(T)x0, (T)x1, (T)x2, (T)x3};
+  if (n >= 4) {
+    memcpy(p, v, sizeof(v));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = v[i];
+  }
+}
+// A column's values (one row of the output in memory): block db of 32 rows of a transposed result.
+template <typename T>
+__device__ __forceinline__ void store_column(T* row, int D, int db, const Acc& x, float f) {
+  const int hi = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int d = db * 32 + 8 * g + 4 * hi;
+    store4(row + d, D - d, x[4 * g] * f, x[4 * g + 1] * f, x[4 * g + 2] * f, x[4 * g + 3] * f);
+  }
+}
+
+// ---- host side ----
+
+// Head sizes are rounded up to a multiple of 32.
+template <typename F>
+inline int by_head(int D, F&& f) {
+  using std::integral_constant;
+  if (D <= 32) return f(integral_constant<int, 32>{});
+  if (D <= 64) return f(integral_constant<int, 64>{});
+  if (D <= 96) return f(integral_constant<int, 96>{});
+  return f(integral_constant<int, 128>{});
+}
+
+// Launches a kernel whose dynamic LDS may pass 64 KB.
+template <typename K>
+inline int launch_lds(K kernel, LdsLimit& lim, int blocks, int threads, size_t lds,
+                      const AttnArgs& a, hipStream_t stream) {
+  if (lds > 64 * 1024)
+    if (const int e = raise_lds_limit(reinterpret_cast<const void*>(kernel), lim)) return e;
+  kernel<<<blocks, threads, lds, stream>>>(a);
+  return launch_status();
+}
+
+constexpr int kAttnFillBlocks = 512;   // two blocks a CU: below this the long axis is split
+constexpr int kAttnMaxSplit = 64;
+
+// Parts of `tiles` steps of the long axis for `blocks` blocks: as many as fill the card, each of
+// `least` steps or more.
+inline int attn_splits(int64_t blocks, int tiles, int least) {
+  if (blocks <= 0 || tiles <= 0) return 1;
+  int64_t n = kAttnFillBlocks / blocks;
+  const int64_t most = tiles / least;
+  n = n < most ? n : most;
+  n = n < kAttnMaxSplit ? n : kAttnMaxSplit;
+  return (int)(n < 1 ? 1 : n);
+}
+
+// Blocks and splits of each kernel for a shape.
+struct AttnPlan {
+  int fw, fs;        // forward: waves a block, splits
+  int qw, qs;        // dq
+  int kw, ks;        // dk, dv
+  int rb_f, rb_q, kb;
+};
+AttnPlan attn_plan(const AttnArgs& a, int BH);
+
+int attn_launch_fwd(const AttnArgs& a, int BH, int dtype, const AttnPlan& p, hipStream_t stream);
+int attn_launch_dq(const AttnArgs& a, int BH, int dtype, const AttnPlan& p, hipStream_t stream);
+int attn_launch_dkv(const AttnArgs& a, int BH, int dtype, const AttnPlan& p, hipStream_t stream);
+
+}  // namespace tts

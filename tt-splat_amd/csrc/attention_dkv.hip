@@ -1,0 +1,384 @@
+// Attention backward, the keys' side: dK and dV; and the C entry points.
+//
+// A wave owns 32 keys (columns of S, dV^T and dK^T): K and V stay in registers as B operands and the
+// rows' Q and dO pass through LDS, 32 rows a tile, with their log-sum-exp, D and (causal) last
+// visible key.  S gives P, dO V^T gives dP; P and dS are the B operands of dV^T += dO^T P and
+// dK^T += Q^T dS, whose A operands are transposed reads of the same tiles.  Rows of all query heads of
+// the group follow one another, so the sum over shared heads is the loop's.
+//
+// Few keys and many rows (gaussians over a view's tokens): the rows are split over blocks, and
+// k_attn_dkv_join adds the parts in order.
+
+#include "attention.h"
+
+namespace tts {
+
+constexpr int kDkvRows = 32;
+
+template <typename T, int DP>
+constexpr size_t dkv_lds() {
+  return (size_t)4 * kDkvRows * kTileStride<T, DP> * sizeof(T) + 2 * 3 * kDkvRows * 4;
+}
+
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attn_dkv(AttnArgs a) {
+  constexpr int KC = DP / 16, DB = DP / 32, BM = kDkvRows, NT = 64 * NW;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int kTile = BM * kTileStride<T, DP>;
+  T* tq = reinterpret_cast<T*>(smem);
+  T* tg = tq + 2 * kTile;
+  float* stat = reinterpret_cast<float*>(tg + 2 * kTile);   // [2][lse2, delta, lim][BM]
+
+  const int nkb = (a.Nk + 32 * NW - 1) / (32 * NW);
+  const int item = xcd_item(blockIdx.x, gridDim.x);
+  const int kb = item % nkb, sp = item / nkb % a.nsplit, bh = item / nkb / a.nsplit;
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
+  const int key0 = kb * 32 * NW, key = key0 + wave * 32 + (lane & 31);
+  const T* qp = static_cast<const T*>(a.q) + b * a.sq.b + (int64_t)hk * a.grp * a.sq.h;
+  const T* gp = static_cast<const T*>(a.dout) + b * a.sdo.b + (int64_t)hk * a.grp * a.sdo.h;
+
+  bool on = key < a.Nk;
+  if (on && a.mask) on = a.mask[b * a.mask_stride + key] != 0;
+  Frag<T> k[KC], v[KC];
+  {
+    const int kk = min(key, a.Nk - 1);
+    const T* kp = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h + kk * a.sk.n;
+    const T* vp = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h + kk * a.sv.n;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int d = c * 16 + hi * 8;
+      k[c] = load_frag(kp + d, on ? a.D - d : 0);
+      v[c] = load_frag(vp + d, on ? a.D - d : 0);
+    }
+  }
+  Acc dk[DB] = {}, dv[DB] = {};
+  const float c2 = a.scale * kLog2e;
+
+  // rows of this part; causal: none before the first that sees the block's first key
+  const int tiles = (a.R + BM - 1) / BM;
+  int t = (int)((int64_t)tiles * sp / a.nsplit);
+  int t1 = (int)((int64_t)tiles * (sp + 1) / a.nsplit);
+  if (a.causal) {
+    const int64_t first = (int64_t)max(key0 - a.off, 0) * a.grp / BM;
+    t = (int)(first > t ? (first < t1 ? first : t1) : t);
+  }
+  {   // no live key in the block: no rows
+    int* any = reinterpret_cast<int*>(stat);
+    const bool some = __ballot(on) != 0;
+    if (lane == 0) any[wave] = some;
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) n |= any[w];
+    __syncthreads();
+    if (!n) t1 = t;
+  }
+
+  TileLoad<T, DP, BM, NT> lq, lg;
+  float st0 = 0.0f, st1 = 0.0f;
+  int st2 = 0;
+  auto fetch = [&](int tile) {
+    lq.load(qp, a.D, [&](int n) {
+      int pos, h;
+      attn_row(a, min(tile * BM + n, a.R - 1), &pos, &h);
+      return row_offset(a.sq, pos, h);
+    });
+    lg.load(gp, a.D, [&](int n) {
+      int pos, h;
+      attn_row(a, min(tile * BM + n, a.R - 1), &pos, &h);
+      return row_offset(a.sdo, pos, h);
+    });
+    if (threadIdx.x < BM) {
+      const int r = tile * BM + threadIdx.x;
+      int pos, h;
+      attn_row(a, min(r, a.R - 1), &pos, &h);
+      st0 = a.lse[((int64_t)b * a.Hkv * a.grp + hk * a.grp + h) * a.Nq + pos] * kLog2e;
+      st1 = a.delta[(int64_t)bh * a.R + min(r, a.R - 1)];
+      st2 = pos + a.off;
+      // rows without a key, and rows past the last: every P is exp2(-inf) = 0
+      if (st0 == -INFINITY || r >= a.R) st0 = INFINITY;
+      if (r >= a.R) st1 = 0.0f;
+    }
+  };
+  auto put = [&](int tile, int buf) {
+    const int n = a.R - tile * BM;
+    const uint64_t rows = n >= BM ? (1ull << BM) - 1 : (1ull << n) - 1;
+    lq.store(tq + buf * kTile, rows, a.D);
+    lg.store(tg + buf * kTile, rows, a.D);
+    if (threadIdx.x < BM) {
+      float* s = stat + buf * 3 * BM;
+      s[threadIdx.x] = st0;
+      s[BM + threadIdx.x] = st1;
+      reinterpret_cast<int*>(s)[2 * BM + threadIdx.x] = st2;
+    }
+  };
+  if (t < t1) {
+    fetch(t);
+    put(t, 0);
+  }
+  int buf = 0;
+  for (; t < t1; ++t) {
+    const bool more = t + 1 < t1;
+    __syncthreads();   // this tile is written, the other buffer is read
+    if (more) fetch(t + 1);
+    const T* sq = tq + buf * kTile;
+    const T* sg = tg + buf * kTile;
+    const float* st = stat + buf * 3 * BM;
+    Acc s = {}, p = {};
+#pragma unroll
+    for (int c = 0; c < KC; ++c) s = mma(tile_frag<T, DP>(sq, 0, c * 16), k[c], s);
+#pragma unroll
+    for (int c = 0; c < KC; ++c) p = mma(tile_frag<T, DP>(sg, 0, c * 16), v[c], p);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 ls = *reinterpret_cast<const float4*>(st + 8 * g + 4 * hi);
+      const float4 de = *reinterpret_cast<const float4*>(st + BM + 8 * g + 4 * hi);
+      const int4 li = *reinterpret_cast<const int4*>(st + 2 * BM + 8 * g + 4 * hi);
+      const float lse2[4] = {ls.x, ls.y, ls.z, ls.w}, delta[4] = {de.x, de.y, de.z, de.w};
+      const int lim[4] = {li.x, li.y, li.z, li.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = 4 * g + j;
+        const bool see = on && (!a.causal || key <= lim[j]);
+        const float e = see ? exp2_(__builtin_fmaf(s[i], c2, -lse2[j])) : 0.0f;
+        s[i] = e;
+        p[i] = e * (p[i] - delta[j]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const Frag<T> pf = acc_frag<T>(s, c), df = acc_frag<T>(p, c);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        dv[d] = mma(transpose_frag<T, DP>(sg, c * 16, d * 32), pf, dv[d]);
+        dk[d] = mma(transpose_frag<T, DP>(sq, c * 16, d * 32), df, dk[d]);
+      }
+    }
+    if (more) put(t + 1, buf ^ 1);
+    buf ^= 1;
+  }
+  if (key >= a.Nk) return;
+  if (a.nsplit == 1) {
+    if (a.dk) {
+      T* kp = static_cast<T*>(a.dk) + b * a.sdk.b + hk * a.sdk.h + key * a.sdk.n;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) store_column(kp, a.D, d, dk[d], a.scale);
+    }
+    if (a.dv) {
+      T* vp = static_cast<T*>(a.dv) + b * a.sdv.b + hk * a.sdv.h + key * a.sdv.n;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) store_column(vp, a.D, d, dv[d], 1.0f);
+    }
+  } else {
+    const int64_t i = (((int64_t)sp * (gridDim.x / nkb / a.nsplit) + bh) * a.Nk + key) * 2;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      store_column(a.part2 + i * a.D, a.D, d, dk[d], a.scale);
+      store_column(a.part2 + (i + 1) * a.D, a.D, d, dv[d], 1.0f);
+    }
+  }
+}
+
+// Sums the parts of split keys, in order: L lanes a (key, dk or dv).
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_dkv_join(AttnArgs a, int BH, int L) {
+  const int lig = threadIdx.x & (L - 1);
+  const int64_t rows = (int64_t)BH * a.Nk * 2;
+  const int64_t i = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  if (i >= rows) return;
+  const int bh = (int)(i / 2 / a.Nk), key = (int)(i / 2 - (int64_t)bh * a.Nk);
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const AttnStride& s = i & 1 ? a.sdv : a.sdk;
+  T* op = static_cast<T*>(i & 1 ? a.dv : a.dk);
+  if (!op) return;
+  op += b * s.b + hk * s.h + key * s.n;
+  for (int c = lig * 4; c < a.D; c += L * 4) {
+    float x[4] = {};
+#pragma unroll 4
+    for (int p = 0; p < a.nsplit; ++p) {
+      float v[4];
+      load_row(a.part2 + (p * rows + i) * a.D + c, a.D - c, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] += v[j];
+    }
+    store4(op + c, a.D - c, x[0], x[1], x[2], x[3]);
+  }
+}
+
+template <typename T, int DP, int NW>
+int launch_dkv(const AttnArgs& a, int blocks, hipStream_t stream) {
+  static LdsLimit lim;
+  return launch_lds(k_attn_dkv<T, DP, NW>, lim, blocks, 64 * NW, dkv_lds<T, DP>(), a, stream);
+}
+
+int attn_launch_dkv(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hipStream_t stream) {
+  AttnArgs a = a0;
+  a.nsplit = p.ks;
+  const int blocks = p.kb * p.ks * BH;
+  return by_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    const int e = by_head(a.D, [&](auto dp) {
+      if (p.kw == 1) return launch_dkv<T, dp(), 1>(a, blocks, stream);
+      return launch_dkv<T, dp(), 2>(a, blocks, stream);
+    });
+    if (e || p.ks == 1) return e;
+    const int L = row_lanes((a.D + 3) / 4);
+    const int64_t rows = (int64_t)BH * a.Nk * 2;
+    k_attn_dkv_join<T><<<(int)((rows * L + 255) / 256), 256, 0, stream>>>(a, BH, L);
+    return launch_status();
+  });
+}
+
+// Up to 32 rows (keys) one wave a block holds them all; past that four waves share the tiles they
+// read.  Then the long axis is split until the card is full.
+AttnPlan attn_plan(const AttnArgs& a, int BH) {
+  AttnPlan p;
+  p.fw = p.qw = a.R <= 32 ? 1 : 4;
+  const int bn = p.fw == 1 ? 32 : 64, tiles = (a.Nk - 1) / bn + 1;
+  p.rb_f = p.rb_q = (a.R - 1) / (32 * p.fw) + 1;
+  p.fs = p.qs = attn_splits((int64_t)p.rb_f * BH, tiles, p.fw == 1 ? 2 : 4);
+  p.kw = a.Nk <= 32 ? 1 : 2;
+  p.kb = (a.Nk - 1) / (32 * p.kw) + 1;
+  p.ks = attn_splits((int64_t)p.kb * BH, (a.R - 1) / kDkvRows + 1, 8);
+  return p;
+}
+
+// Sub-buffers of the workspaces: forward's parts; backward's D, then parts of dQ and of dK, dV.
+size_t attn_fwd_layout(AttnArgs& a, int64_t BH, const AttnPlan& p, char* base) {
+  if (p.fs == 1) return 0;
+  const size_t o = align256((size_t)p.fs * BH * a.R * a.D * sizeof(float));
+  a.part = reinterpret_cast<float*>(base);
+  a.part2 = reinterpret_cast<float*>(base + o);
+  return o + align256((size_t)p.fs * BH * a.R * sizeof(float));
+}
+size_t attn_bwd_layout(AttnArgs& a, int64_t BH, const AttnPlan& p, char* base) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* r = base + off;
+    off += align256(bytes);
+    return reinterpret_cast<float*>(r);
+  };
+  a.delta = take((size_t)BH * a.R * sizeof(float));
+  a.part = take(p.qs > 1 ? (size_t)p.qs * BH * a.R * a.D * sizeof(float) : 0);
+  a.part2 = take(p.ks > 1 ? (size_t)p.ks * BH * a.Nk * 2 * a.D * sizeof(float) : 0);
+  return off;
+}
+
+// Checks a shape's numbers and sets what both directions take from it.
+int attn_shape(const tts_attention_shape* s, AttnArgs* a, int* BH) {
+  if (s->batch < 0 || s->kv_heads < 1 || s->heads < 1 || s->queries < 0 || s->keys < 0 ||
+      !(s->scale > 0.0) || !(s->scale < 3.0e38))
+    return TTS_EINVAL;
+  if (s->head_dim < 1 || s->head_dim > 128 || s->heads % s->kv_heads) return TTS_EHEADS;
+  if (s->dtype < 0 || s->dtype > 2) return TTS_EDTYPE;
+  const int64_t grp = s->heads / s->kv_heads, lim = (int64_t)1 << 30;
+  if (grp > lim || s->queries > lim / grp || s->keys > lim || s->batch > lim ||
+      s->kv_heads > lim || (s->batch > 0 && s->kv_heads > lim / s->batch))
+    return TTS_ELENGTH;
+  *a = AttnArgs{};
+  auto st = [](const int64_t* x) { return AttnStride{x[0], x[1], x[2]}; };
+  a->sq = st(s->q);
+  a->sk = st(s->k);
+  a->sv = st(s->v);
+  a->so = st(s->o);
+  a->sdo = st(s->dout);
+  a->sdq = st(s->dq);
+  a->sdk = st(s->dk);
+  a->sdv = st(s->dv);
+  a->mask_stride = s->mask_stride;
+  a->Hkv = (int)s->kv_heads;
+  a->grp = (int)grp;
+  a->Nq = (int)s->queries;
+  a->Nk = (int)s->keys;
+  a->D = (int)s->head_dim;
+  a->R = (int)(s->queries * grp);
+  a->causal = s->causal != 0;
+  a->off = (int)(s->keys - s->queries);
+  a->scale = (float)s->scale;
+  *BH = (int)(s->batch * s->kv_heads);
+  return TTS_OK;
+}
+
+// Blocks of a launch are 32-bit.
+bool attn_fits(const AttnArgs& a, int64_t BH, const AttnPlan& p) {
+  const int64_t lim = (int64_t)1 << 30;
+  return (int64_t)p.rb_f * p.fs * BH < lim && (int64_t)p.kb * p.ks * BH < lim &&
+         BH * a.R < lim && BH * a.Nk < lim;
+}
+
+}  // namespace tts
+
+using namespace tts;
+
+extern "C" {
+
+size_t tts_attention_workspace_bytes(const tts_attention_shape* shape, int backward) {
+  AttnArgs a;
+  int BH;
+  if (!shape || attn_shape(shape, &a, &BH) || !BH || !a.R || !a.Nk) return 0;
+  const AttnPlan p = attn_plan(a, BH);
+  return backward ? attn_bwd_layout(a, BH, p, nullptr) : attn_fwd_layout(a, BH, p, nullptr);
+}
+
+int tts_attention_fwd(const tts_attention_shape* shape, const void* q, const void* k,
+                      const void* v, const uint8_t* key_mask, void* out, float* lse,
+                      void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (!shape) return TTS_EINVAL;
+  AttnArgs a;
+  int BH;
+  if (const int e = attn_shape(shape, &a, &BH)) return e;
+  if (!BH || !a.R) return TTS_OK;
+  if (!q || !out || (a.Nk > 0 && (!k || !v))) return TTS_EINVAL;
+  AttnPlan p = {};
+  if (a.Nk > 0) {
+    p = attn_plan(a, BH);
+  } else {   // no keys: rows of zeros, no tile is read
+    p.fw = 4;
+    p.rb_f = (a.R - 1) / 128 + 1;
+    p.fs = 1;
+    p.kb = p.ks = 1;
+    key_mask = nullptr;
+  }
+  if (!attn_fits(a, BH, p)) return TTS_ELENGTH;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.mask = key_mask;
+  a.out = out;
+  a.lse = lse;
+  const size_t need = attn_fwd_layout(a, BH, p, static_cast<char*>(workspace));
+  if (need && (!workspace || workspace_bytes < need)) return TTS_EWORKSPACE;
+  return attn_launch_fwd(a, BH, (int)shape->dtype, p, stream);
+}
+
+int tts_attention_bwd(const tts_attention_shape* shape, const void* q, const void* k,
+                      const void* v, const uint8_t* key_mask, const void* out, const float* lse,
+                      const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream) {
+  if (!shape) return TTS_EINVAL;
+  AttnArgs a;
+  int BH;
+  if (const int e = attn_shape(shape, &a, &BH)) return e;
+  if (!BH || !a.R || !a.Nk) return TTS_EINVAL;   // no product to differentiate
+  if (!q || !k || !v || !out || !lse || !dout || (!dq && !dk && !dv)) return TTS_EINVAL;
+  const AttnPlan p = attn_plan(a, BH);
+  if (!attn_fits(a, BH, p)) return TTS_ELENGTH;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.mask = key_mask;
+  a.o = out;
+  a.lse = const_cast<float*>(lse);
+  a.dout = dout;
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  const size_t need = attn_bwd_layout(a, BH, p, static_cast<char*>(workspace));
+  if (!workspace || workspace_bytes < need) return TTS_EWORKSPACE;
+  if (const int e = attn_launch_dq(a, BH, (int)shape->dtype, p, stream)) return e;
+  if (!dk && !dv) return TTS_OK;
+  return attn_launch_dkv(a, BH, (int)shape->dtype, p, stream);
+}
+
+}  // extern "C"

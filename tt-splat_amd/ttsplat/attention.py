@@ -1,0 +1,49 @@
+"""Attention on the GPU (no counterpart in the reference): gaussians over a view's tokens, tokens
+among themselves.
+
+`attention(q, k, v, key_mask, causal, scale)` is differentiable w.r.t. q, k and v.  The forward
+keeps each row's log-sum-exp and no scores; the backward recomputes the probabilities.  Types
+fp32, fp16 and bf16; the softmax and all sums are fp32.  Results are the same bits every time.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import kernels
+
+F32 = torch.float32
+
+
+def _last_contiguous(t):
+    return t if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[3] < 2 \
+        or t.stride(3) == 1 else t.contiguous()
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, key_mask, causal, scale):
+        lse = torch.empty(q.shape[:3], device=q.device, dtype=F32)
+        out = kernels.attention_fwd(q, k, v, key_mask, causal, scale, lse=lse)
+        ctx.save_for_backward(q, k, v, key_mask, out, lse)
+        ctx.meta = (causal, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, key_mask, out, lse = ctx.saved_tensors
+        nq, nk, nv = ctx.needs_input_grad[:3]
+        grads = kernels.attention_bwd(q, k, v, out, lse, _last_contiguous(dout), key_mask, *ctx.meta,
+                                      nq, nk, nv)
+        return (*grads, None, None, None)
+
+
+def attention(q, k, v, key_mask=None, causal=False, scale=None):
+    """softmax(scale q k^T) v.  q [B, Hq, Nq, D], k and v [B, Hkv, Nk, D]: query head h reads key
+    head h / (Hq / Hkv); any strides ([B, N, H, D] memory as a transposed view needs no copy), D up
+    to 128, scale 1/sqrt(D) unless given.  key_mask [B, Nk] bool or uint8: False hides a key (a
+    gaussian out of view, padding), whatever its k and v hold.  causal: row i sees keys up to
+    i + Nk - Nq.  A row that sees no key gives zeros and no gradient."""
+    q, k, v = _last_contiguous(q), _last_contiguous(k), _last_contiguous(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attention.apply(q, k, v, key_mask, bool(causal), scale)
+    return kernels.attention_fwd(q, k, v, key_mask, causal, scale)

@@ -5,6 +5,8 @@ kernel on the current torch stream.  Nothing here allocates unless an output is 
 (out=None); the graph-captured training step passes every buffer in.
 """
 import ctypes
+import math
+import struct
 
 import torch
 
@@ -1151,3 +1153,104 @@ def embedding_bwd(dout, ids, V, scale=1.0, out=None, workspace=None):
     call("tts_embedding_bwd", ptr(dout), ptr(ids), wide, N, V, D, float(scale), code, ptr(out),
          ptr(workspace), workspace.numel(), stream())
     return out
+
+
+_ATTN_SHAPE = struct.Struct("=33qd")   # tts_attention_shape
+_NO_STRIDE = (0, 0, 0)
+
+
+def _attn_tensor(t, name, shape=None, dtype=None, device=None):
+    code = _elem(t, name, device, dtype)
+    if t.dim() != 4:
+        raise ValueError(f"{name} must be [batch, heads, length, head_dim], got {tuple(t.shape)}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    st = t.stride()
+    if st[3] != 1 and t.shape[3] > 1:
+        raise ValueError(f"{name} must have a contiguous last axis")
+    return code, st[:3]
+
+
+def _attn_args(q, k, v, key_mask, causal, scale, out, dout=None, grads=(None, None, None)):
+    """The call's shape block, checked, and the mask as uint8."""
+    code, sq = _attn_tensor(q, "q")
+    dev, dt = q.device, q.dtype
+    _, sk = _attn_tensor(k, "k", None, dt, dev)
+    B, Hq, Nq, D = q.shape
+    _, Hkv, Nk, _ = k.shape
+    if k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"k has shape {tuple(k.shape)}, expected [{B}, heads, keys, {D}]")
+    _, sv = _attn_tensor(v, "v", k.shape, dt, dev)
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads are not a multiple of {Hkv} key heads")
+    if not 1 <= D <= 128:
+        raise ValueError(f"head size must be in [1, 128], got {D}")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    _, so = _attn_tensor(out, "out", q.shape, dt, dev)
+    ms = 0
+    if key_mask is not None:
+        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in (torch.bool, U8):
+            raise ValueError("key_mask must be a bool or uint8 tensor")
+        if key_mask.device != dev or key_mask.shape != (B, Nk):
+            raise ValueError(f"key_mask must be [{B}, {Nk}] on {dev}, got "
+                             f"{tuple(key_mask.shape)} on {key_mask.device}")
+        if key_mask.dtype == torch.bool:
+            key_mask = key_mask.view(U8)
+        if Nk > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+        ms = key_mask.stride(0)
+    sdo = _NO_STRIDE if dout is None else _attn_tensor(dout, "dout", q.shape, dt, dev)[1]
+    sg = [_NO_STRIDE if g is None else _attn_tensor(g, n, t.shape, dt, dev)[1]
+          for g, n, t in zip(grads, ("dq", "dk", "dv"), (q, k, v))]
+    return _ATTN_SHAPE.pack(B, Hq, Hkv, Nq, Nk, D, 1 if causal else 0, code, ms, *sq, *sk, *sv, *so,
+                            *sdo, *sg[0], *sg[1], *sg[2], scale), key_mask
+
+
+def _attn_like(t):
+    """A new tensor in t's order of axes where that keeps the last one contiguous."""
+    r = torch.empty_like(t)
+    return r if r.dim() != 4 or r.shape[3] < 2 or r.stride(3) == 1 else torch.empty(
+        t.shape, device=t.device, dtype=t.dtype)
+
+
+def _attn_workspace(shape, backward, device):
+    n = _lib.load().tts_attention_workspace_bytes(shape, backward)
+    return (torch.empty(n, device=device, dtype=U8), n) if n else (None, 0)
+
+
+def attention_fwd(q, k, v, key_mask=None, causal=False, scale=None, out=None, lse=None):
+    """out [B, Hq, Nq, D] = softmax(scale q k^T) v over the keys that key_mask [B, Nk] (non-zero:
+    visible) and causal (row i sees keys up to i + Nk - Nq) leave; rows without a key give zeros.
+    q [B, Hq, Nq, D], k and v [B, Hkv, Nk, D], Hq a multiple of Hkv, any strides with a contiguous
+    last axis.  lse [B, Hq, Nq] fp32, when given, takes each row's log-sum-exp."""
+    out = _attn_like(q) if out is None else out
+    shape, mask = _attn_args(q, k, v, key_mask, causal, scale, out)
+    if lse is not None:
+        require(lse, "lse", F32, q.shape[:3], q.device)
+    ws, n = _attn_workspace(shape, 0, q.device)
+    call("tts_attention_fwd", shape, ptr(q), ptr(k), ptr(v), ptr(mask), ptr(out), ptr(lse), ptr(ws),
+         n, stream())
+    return out
+
+
+def attention_bwd(q, k, v, out, lse, dout, key_mask=None, causal=False, scale=None, need_dq=True,
+                  need_dk=True, need_dv=True):
+    """(dq, dk, dv) from the forward's out and lse; a part that is not needed is None."""
+    dq = _attn_like(q) if need_dq else None
+    dk = _attn_like(k) if need_dk else None
+    dv = _attn_like(v) if need_dv else None
+    shape, mask = _attn_args(q, k, v, key_mask, causal, scale, out, dout, (dq, dk, dv))
+    require(lse, "lse", F32, q.shape[:3], q.device)
+    if not (need_dq or need_dk or need_dv):
+        return None, None, None
+    if q.shape[0] * q.shape[2] * k.shape[2] == 0:      # no score: no gradient
+        for g in (dq, dk, dv):
+            if g is not None:
+                g.zero_()
+        return dq, dk, dv
+    ws, n = _attn_workspace(shape, 1, q.device)
+    call("tts_attention_bwd", shape, ptr(q), ptr(k), ptr(v), ptr(mask), ptr(out), ptr(lse),
+         ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(ws), n, stream())
+    return dq, dk, dv
