@@ -46,9 +46,10 @@ __device__ __forceinline__ Acc mma(Frag<float> a, Frag<float> b, Acc c) {
   return c;
 }
 
-// Strides in elements of (batch, head, row).
+// Strides in elements of (batch, head, row); a row's is below 2^31, its product with a row is 64-bit.
 struct AttnStride {
-  int64_t b, h, n;
+  int64_t b, h;
+  int n;
 };
 
 struct AttnArgs {
@@ -75,7 +76,7 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, int r, int* pos, int
   }
 }
 __device__ __forceinline__ int64_t row_offset(const AttnStride& s, int pos, int h) {
-  return h * s.h + pos * s.n;
+  return h * s.h + (int64_t)pos * s.n;
 }
 
 // Eight values at p, n of them within the row, zeros behind.
@@ -89,6 +90,19 @@ __device__ __forceinline__ Frag<T> load_frag(const T* p, int n) {
     for (int i = 0; i < 8; ++i) f[i] = i < n ? p[i] : (T)0.0f;
   }
   return f;
+}
+
+// Waits here for a value that was loaded, so that its first use inside a loop does not: that wait would
+// be for every load that is in flight there, the next tile's among them.
+template <typename F>
+__device__ __forceinline__ void arrive(F& f) {
+  constexpr int N = sizeof(F) / 16;
+  using V4 = int __attribute__((ext_vector_type(4)));
+  V4 v[N];
+  memcpy(v, &f, sizeof(F));
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
+  memcpy(&f, v, sizeof(F));
 }
 
 // Tiles in LDS: row-major, rows 16 bytes longer than their data, which spreads the rows of one
@@ -133,27 +147,27 @@ __device__ __forceinline__ Frag<T> transpose_frag(const T* tile, int row0, int d
 
 // One tile of BN rows on its way from memory to LDS through registers: load() starts the reads, store()
 // writes the tile, zeros for rows not in `live` (masked and missing keys: whatever stands there, NaN
-// among it, stays out of the products) and past the head size.
-template <typename T, int DP, int BN, int NT>
+// among it, stays out of the products) and past the head size.  ODD: head sizes that are no multiple
+// of eight, read value by value; a branch for them in the same kernel makes the compiler wait for
+// the loads at once, which costs the overlap (2500 x 2500 bf16 forward 95 -> TODO us).
+template <typename T, int DP, int BN, int NT, bool ODD>
 struct TileLoad {
   static constexpr int kPerRow = DP / 8, kN = BN * kPerRow / NT;
   static_assert(kN * NT == BN * kPerRow, "threads must divide the tile");
   Frag<T> r[kN];
 
-  // row(i): offset of the tile's row i (any valid row for rows that are not live)
+  // row(i): pointer to the tile's row i (any valid row for rows that are not live)
   template <typename Row>
-  __device__ __forceinline__ void load(const T* base, int D, Row row) {
-    if ((D & 7) == 0) {
+  __device__ __forceinline__ void load(int D, Row row) {
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int v = threadIdx.x + i * NT, d0 = v % kPerRow * 8;
-        memcpy(&r[i], base + row(v / kPerRow) + (d0 < D ? d0 : 0), 8 * sizeof(T));
-      }
-    } else {
+    for (int i = 0; i < kN; ++i) {
+      const int v = threadIdx.x + i * NT, d0 = v % kPerRow * 8;
+      const T* p = row(v / kPerRow);
+      if constexpr (ODD) {
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int v = threadIdx.x + i * NT, d0 = v % kPerRow * 8;
-        r[i] = load_frag(base + row(v / kPerRow) + d0, D - d0);
+        for (int j = 0; j < 8; ++j) r[i][j] = p[d0 + j < D ? d0 + j : 0];
+      } else {
+        memcpy(&r[i], p + (d0 < D ? d0 : 0), 8 * sizeof(T));
       }
     }
   }
@@ -164,7 +178,7 @@ struct TileLoad {
       const bool on = ((live >> n) & 1) && d0 < D;
       Frag<T> f = r[i];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = on ? f[j] : (T)0.0f;
+      for (int j = 0; j < 8; ++j) f[j] = on && (!ODD || d0 + j < D) ? f[j] : (T)0.0f;
       memcpy(__builtin_assume_aligned(tile + n * kTileStride<T, DP> + d0, 16), &f, 8 * sizeof(T));
     }
   }
@@ -282,6 +296,21 @@ __device__ __forceinline__ void store4(T* p, int n, float x0, float x1, float x2
       if (i < n) p[i] = v[i];
   }
 }
+// The result's accumulators set to base[row], as the products' start.
+__device__ __forceinline__ Acc acc_rows(const float* base) {
+  const int hi = (threadIdx.x & 63) >> 5;
+  Acc s;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const float4 x = *reinterpret_cast<const float4*>(base + 8 * g + 4 * hi);
+    s[4 * g] = x.x;
+    s[4 * g + 1] = x.y;
+    s[4 * g + 2] = x.z;
+    s[4 * g + 3] = x.w;
+  }
+  return s;
+}
+
 // A column's values (one row of the output in memory): block db of 32 rows of a transposed result.
 template <typename T>
 __device__ __forceinline__ void store_column(T* row, int D, int db, const Acc& x, float f) {
@@ -295,14 +324,19 @@ __device__ __forceinline__ void store_column(T* row, int D, int db, const Acc& x
 
 // ---- host side ----
 
-// Head sizes are rounded up to a multiple of 32.
+// Head sizes are rounded up to a multiple of 32; those that are no multiple of eight, to 32 or 128.
 template <typename F>
 inline int by_head(int D, F&& f) {
+  using std::bool_constant;
   using std::integral_constant;
-  if (D <= 32) return f(integral_constant<int, 32>{});
-  if (D <= 64) return f(integral_constant<int, 64>{});
-  if (D <= 96) return f(integral_constant<int, 96>{});
-  return f(integral_constant<int, 128>{});
+  if (D & 7) {
+    if (D <= 32) return f(integral_constant<int, 32>{}, bool_constant<true>{});
+    return f(integral_constant<int, 128>{}, bool_constant<true>{});
+  }
+  if (D <= 32) return f(integral_constant<int, 32>{}, bool_constant<false>{});
+  if (D <= 64) return f(integral_constant<int, 64>{}, bool_constant<false>{});
+  if (D <= 96) return f(integral_constant<int, 96>{}, bool_constant<false>{});
+  return f(integral_constant<int, 128>{}, bool_constant<false>{});
 }
 
 // Launches a kernel whose dynamic LDS may pass 64 KB.

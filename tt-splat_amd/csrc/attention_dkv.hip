@@ -13,21 +13,21 @@
 
 namespace tts {
 
-constexpr int kDkvRows = 32;
+constexpr int kDkvRows = 64;   // rows a tile with four waves a block
 
-template <typename T, int DP>
+template <typename T, int DP, int BM>
 constexpr size_t dkv_lds() {
-  return (size_t)4 * kDkvRows * kTileStride<T, DP> * sizeof(T) + 2 * 3 * kDkvRows * 4;
+  return (size_t)4 * BM * kTileStride<T, DP> * sizeof(T) + 2 * 3 * BM * sizeof(float);
 }
 
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) void k_attn_dkv(AttnArgs a) {
-  constexpr int KC = DP / 16, DB = DP / 32, BM = kDkvRows, NT = 64 * NW;
+template <typename T, int DP, int NW, int BM, bool ODD>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
+  constexpr int KC = DP / 16, DB = DP / 32, NT = 64 * NW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int kTile = BM * kTileStride<T, DP>;
   T* tq = reinterpret_cast<T*>(smem);
   T* tg = tq + 2 * kTile;
-  float* stat = reinterpret_cast<float*>(tg + 2 * kTile);   // [2][lse2, delta, lim][BM]
+  float* stat = reinterpret_cast<float*>(tg + 2 * kTile);   // [2][-L / scale, -D, last key][BM]
 
   const int nkb = (a.Nk + 32 * NW - 1) / (32 * NW);
   const int item = xcd_item(blockIdx.x, gridDim.x);
@@ -40,9 +40,10 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(AttnArgs a) {
 
   bool on = key < a.Nk;
   if (on && a.mask) on = a.mask[b * a.mask_stride + key] != 0;
+  const bool busy = __ballot(on) != 0;   // the wave has a live key
   Frag<T> k[KC], v[KC];
   {
-    const int kk = min(key, a.Nk - 1);
+    const int64_t kk = min(key, a.Nk - 1);
     const T* kp = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h + kk * a.sk.n;
     const T* vp = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h + kk * a.sv.n;
 #pragma unroll
@@ -51,9 +52,14 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(AttnArgs a) {
       k[c] = load_frag(kp + d, on ? a.D - d : 0);
       v[c] = load_frag(vp + d, on ? a.D - d : 0);
     }
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      arrive(k[c]);
+      arrive(v[c]);
+    }
   }
   Acc dk[DB] = {}, dv[DB] = {};
-  const float c2 = a.scale * kLog2e;
+  const float c2 = a.scale * kLog2e, inv_scale = 1.0f / a.scale;
 
   // rows of this part; causal: none before the first that sees the block's first key
   const int tiles = (a.R + BM - 1) / BM;
@@ -65,8 +71,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(AttnArgs a) {
   }
   {   // no live key in the block: no rows
     int* any = reinterpret_cast<int*>(stat);
-    const bool some = __ballot(on) != 0;
-    if (lane == 0) any[wave] = some;
+    if (lane == 0) any[wave] = busy;
     __syncthreads();
     int n = 0;
 #pragma unroll
@@ -75,41 +80,38 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(AttnArgs a) {
     if (!n) t1 = t;
   }
 
-  TileLoad<T, DP, BM, NT> lq, lg;
+  TileLoad<T, DP, BM, NT, ODD> lq, lg;
   float st0 = 0.0f, st1 = 0.0f;
   int st2 = 0;
   auto fetch = [&](int tile) {
-    lq.load(qp, a.D, [&](int n) {
+    lq.load(a.D, [&](int n) {
       int pos, h;
       attn_row(a, min(tile * BM + n, a.R - 1), &pos, &h);
-      return row_offset(a.sq, pos, h);
+      return qp + row_offset(a.sq, pos, h);
     });
-    lg.load(gp, a.D, [&](int n) {
+    lg.load(a.D, [&](int n) {
       int pos, h;
       attn_row(a, min(tile * BM + n, a.R - 1), &pos, &h);
-      return row_offset(a.sdo, pos, h);
+      return gp + row_offset(a.sdo, pos, h);
     });
-    if (threadIdx.x < BM) {
-      const int r = tile * BM + threadIdx.x;
-      int pos, h;
-      attn_row(a, min(r, a.R - 1), &pos, &h);
-      st0 = a.lse[((int64_t)b * a.Hkv * a.grp + hk * a.grp + h) * a.Nq + pos] * kLog2e;
-      st1 = a.delta[(int64_t)bh * a.R + min(r, a.R - 1)];
-      st2 = pos + a.off;
-      // rows without a key, and rows past the last: every P is exp2(-inf) = 0
-      if (st0 == -INFINITY || r >= a.R) st0 = INFINITY;
-      if (r >= a.R) st1 = 0.0f;
-    }
+    const int r = min(tile * BM + (int)(threadIdx.x & (BM - 1)), a.R - 1);
+    int pos, h;
+    attn_row(a, r, &pos, &h);
+    st0 = a.lse[((int64_t)b * a.Hkv * a.grp + hk * a.grp + h) * a.Nq + pos];
+    st1 = a.delta[(int64_t)bh * a.R + r];
+    st2 = pos + a.off;
   };
   auto put = [&](int tile, int buf) {
     const int n = a.R - tile * BM;
-    const uint64_t rows = n >= BM ? (1ull << BM) - 1 : (1ull << n) - 1;
+    const uint64_t rows = n >= BM ? (BM == 64 ? ~0ull : (1ull << (BM & 63)) - 1) : (1ull << n) - 1;
     lq.store(tq + buf * kTile, rows, a.D);
     lg.store(tg + buf * kTile, rows, a.D);
     if (threadIdx.x < BM) {
       float* s = stat + buf * 3 * BM;
-      s[threadIdx.x] = st0;
-      s[BM + threadIdx.x] = st1;
+      // rows without a key (L = -inf) and rows past the last: every P is exp2(-inf) = 0
+      const bool none = st0 == -INFINITY || (int)threadIdx.x >= n;
+      s[threadIdx.x] = none ? -INFINITY : -st0 * inv_scale;
+      s[BM + threadIdx.x] = (int)threadIdx.x >= n ? 0.0f : -st1;
       reinterpret_cast<int*>(s)[2 * BM + threadIdx.x] = st2;
     }
   };
@@ -125,48 +127,55 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(AttnArgs a) {
     const T* sq = tq + buf * kTile;
     const T* sg = tg + buf * kTile;
     const float* st = stat + buf * 3 * BM;
-    Acc s = {}, p = {};
+    if (busy) {
 #pragma unroll
-    for (int c = 0; c < KC; ++c) s = mma(tile_frag<T, DP>(sq, 0, c * 16), k[c], s);
+      for (int rb = 0; rb < BM; rb += 32) {
+        // S starts from -L / scale: no subtraction after it.  dP does not start from -D: its sum and D's
+        // are the same terms in the same order for a row with one key, and dS = 0 (row_dots)
+        Acc s = acc_rows(st + rb), p = {};
 #pragma unroll
-    for (int c = 0; c < KC; ++c) p = mma(tile_frag<T, DP>(sg, 0, c * 16), v[c], p);
+        for (int c = 0; c < KC; ++c) s = mma(tile_frag<T, DP>(sq, rb, c * 16), k[c], s);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const float4 ls = *reinterpret_cast<const float4*>(st + 8 * g + 4 * hi);
-      const float4 de = *reinterpret_cast<const float4*>(st + BM + 8 * g + 4 * hi);
-      const int4 li = *reinterpret_cast<const int4*>(st + 2 * BM + 8 * g + 4 * hi);
-      const float lse2[4] = {ls.x, ls.y, ls.z, ls.w}, delta[4] = {de.x, de.y, de.z, de.w};
-      const int lim[4] = {li.x, li.y, li.z, li.w};
+        for (int c = 0; c < KC; ++c) p = mma(tile_frag<T, DP>(sg, rb, c * 16), v[c], p);
+        if (a.causal) {
+          const Acc lim = acc_rows(st + 2 * BM + rb);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = 4 * g + j;
-        const bool see = on && (!a.causal || key <= lim[j]);
-        const float e = see ? exp2_(__builtin_fmaf(s[i], c2, -lse2[j])) : 0.0f;
-        s[i] = e;
-        p[i] = e * (p[i] - delta[j]);
-      }
-    }
+          for (int i = 0; i < 16; ++i)
+            if (key > __builtin_bit_cast(int, (float)lim[i])) s[i] = -INFINITY;
+        }
+        const Acc md = acc_rows(st + BM + rb);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const Frag<T> pf = acc_frag<T>(s, c), df = acc_frag<T>(p, c);
+        for (int i = 0; i < 16; ++i) {
+          s[i] = exp2_(s[i] * c2);
+          p[i] = (p[i] + md[i]) * s[i];
+        }
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        dv[d] = mma(transpose_frag<T, DP>(sg, c * 16, d * 32), pf, dv[d]);
-        dk[d] = mma(transpose_frag<T, DP>(sq, c * 16, d * 32), df, dk[d]);
+        for (int c = 0; c < 2; ++c) {
+          const Frag<T> pf = acc_frag<T>(s, c), df = acc_frag<T>(p, c);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            dv[d] = mma(transpose_frag<T, DP>(sg, rb + c * 16, d * 32), pf, dv[d]);
+            dk[d] = mma(transpose_frag<T, DP>(sq, rb + c * 16, d * 32), df, dk[d]);
+          }
+        }
       }
     }
     if (more) put(t + 1, buf ^ 1);
     buf ^= 1;
   }
+  if (!on) {   // a hidden key's column holds products with zeros
+#pragma unroll
+    for (int d = 0; d < DB; ++d) dk[d] = dv[d] = Acc{};
+  }
   if (key >= a.Nk) return;
   if (a.nsplit == 1) {
     if (a.dk) {
-      T* kp = static_cast<T*>(a.dk) + b * a.sdk.b + hk * a.sdk.h + key * a.sdk.n;
+      T* kp = static_cast<T*>(a.dk) + b * a.sdk.b + hk * a.sdk.h + (int64_t)key * a.sdk.n;
 #pragma unroll
       for (int d = 0; d < DB; ++d) store_column(kp, a.D, d, dk[d], a.scale);
     }
     if (a.dv) {
-      T* vp = static_cast<T*>(a.dv) + b * a.sdv.b + hk * a.sdv.h + key * a.sdv.n;
+      T* vp = static_cast<T*>(a.dv) + b * a.sdv.b + hk * a.sdv.h + (int64_t)key * a.sdv.n;
 #pragma unroll
       for (int d = 0; d < DB; ++d) store_column(vp, a.D, d, dv[d], 1.0f);
     }
@@ -192,7 +201,7 @@ __global__ __launch_bounds__(256) void k_attn_dkv_join(AttnArgs a, int BH, int L
   const AttnStride& s = i & 1 ? a.sdv : a.sdk;
   T* op = static_cast<T*>(i & 1 ? a.dv : a.dk);
   if (!op) return;
-  op += b * s.b + hk * s.h + key * s.n;
+  op += b * s.b + hk * s.h + (int64_t)key * s.n;
   for (int c = lig * 4; c < a.D; c += L * 4) {
     float x[4] = {};
 #pragma unroll 4
@@ -206,10 +215,11 @@ __global__ __launch_bounds__(256) void k_attn_dkv_join(AttnArgs a, int BH, int L
   }
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, int BM, bool ODD>
 int launch_dkv(const AttnArgs& a, int blocks, hipStream_t stream) {
   static LdsLimit lim;
-  return launch_lds(k_attn_dkv<T, DP, NW>, lim, blocks, 64 * NW, dkv_lds<T, DP>(), a, stream);
+  return launch_lds(k_attn_dkv<T, DP, NW, BM, ODD>, lim, blocks, 64 * NW, dkv_lds<T, DP, BM>(), a,
+                    stream);
 }
 
 int attn_launch_dkv(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hipStream_t stream) {
@@ -218,9 +228,10 @@ int attn_launch_dkv(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hi
   const int blocks = p.kb * p.ks * BH;
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const int e = by_head(a.D, [&](auto dp) {
-      if (p.kw == 1) return launch_dkv<T, dp(), 1>(a, blocks, stream);
-      return launch_dkv<T, dp(), 2>(a, blocks, stream);
+    const int e = by_head(a.D, [&](auto dp, auto odd) {
+      if constexpr (!odd())
+        if (p.kw == 1) return launch_dkv<T, dp(), 1, 32, false>(a, blocks, stream);
+      return launch_dkv<T, dp(), 4, kDkvRows, odd()>(a, blocks, stream);
     });
     if (e || p.ks == 1) return e;
     const int L = row_lanes((a.D + 3) / 4);
@@ -234,13 +245,13 @@ int attn_launch_dkv(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hi
 // read.  Then the long axis is split until the card is full.
 AttnPlan attn_plan(const AttnArgs& a, int BH) {
   AttnPlan p;
-  p.fw = p.qw = a.R <= 32 ? 1 : 4;
+  p.fw = p.qw = a.R <= 32 && a.D % 8 == 0 ? 1 : 4;
   const int bn = p.fw == 1 ? 32 : 64, tiles = (a.Nk - 1) / bn + 1;
   p.rb_f = p.rb_q = (a.R - 1) / (32 * p.fw) + 1;
   p.fs = p.qs = attn_splits((int64_t)p.rb_f * BH, tiles, p.fw == 1 ? 2 : 4);
-  p.kw = a.Nk <= 32 ? 1 : 2;
+  p.kw = a.Nk <= 32 && a.D % 8 == 0 ? 1 : 4;
   p.kb = (a.Nk - 1) / (32 * p.kw) + 1;
-  p.ks = attn_splits((int64_t)p.kb * BH, (a.R - 1) / kDkvRows + 1, 8);
+  p.ks = attn_splits((int64_t)p.kb * BH, (a.R - 1) / (p.kw == 1 ? 32 : kDkvRows) + 1, 2);
   return p;
 }
 
@@ -277,7 +288,9 @@ int attn_shape(const tts_attention_shape* s, AttnArgs* a, int* BH) {
       s->kv_heads > lim || (s->batch > 0 && s->kv_heads > lim / s->batch))
     return TTS_ELENGTH;
   *a = AttnArgs{};
-  auto st = [](const int64_t* x) { return AttnStride{x[0], x[1], x[2]}; };
+  for (const int64_t* x : {s->q, s->k, s->v, s->o, s->dout, s->dq, s->dk, s->dv})
+    if (x[2] < 0 || x[2] >= (int64_t)1 << 31) return TTS_ELENGTH;
+  auto st = [](const int64_t* x) { return AttnStride{x[0], x[1], (int)x[2]}; };
   a->sq = st(s->q);
   a->sk = st(s->k);
   a->sv = st(s->v);

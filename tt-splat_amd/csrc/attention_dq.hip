@@ -14,16 +14,17 @@ namespace tts {
 
 template <typename T, int DP, int BN>
 constexpr size_t dq_lds() {
-  return (size_t)4 * BN * kTileStride<T, DP> * sizeof(T);
+  return (size_t)4 * BN * kTileStride<T, DP> * sizeof(T) + 2 * BN * sizeof(float);
 }
 
-template <typename T, int DP, int NW, int BN>
-__global__ __launch_bounds__(64 * NW) void k_attn_dq(AttnArgs a) {
+template <typename T, int DP, int NW, int BN, bool ODD>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2 : 1) void k_attn_dq(AttnArgs a) {
   constexpr int KC = DP / 16, DB = DP / 32, KB = BN / 32, NT = 64 * NW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* tk = reinterpret_cast<T*>(smem);
   constexpr int kTile = BN * kTileStride<T, DP>;
   T* tv = tk + 2 * kTile;
+  float* bias = reinterpret_cast<float*>(tv + 2 * kTile);   // [2][BN] 0, or -inf for hidden keys
 
   const int nrb = (a.R + 32 * NW - 1) / (32 * NW);
   const int item = xcd_item(blockIdx.x, gridDim.x);
@@ -40,9 +41,9 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(AttnArgs a) {
   Frag<T> q[KC], go[KC];
   float delta;
   {
-    const T* qp = static_cast<const T*>(a.q) + b * a.sq.b + hq * a.sq.h + pos * a.sq.n;
-    const T* gp = static_cast<const T*>(a.dout) + b * a.sdo.b + hq * a.sdo.h + pos * a.sdo.n;
-    const T* op = static_cast<const T*>(a.o) + b * a.so.b + hq * a.so.h + pos * a.so.n;
+    const T* qp = static_cast<const T*>(a.q) + b * a.sq.b + hq * a.sq.h + (int64_t)pos * a.sq.n;
+    const T* gp = static_cast<const T*>(a.dout) + b * a.sdo.b + hq * a.sdo.h + (int64_t)pos * a.sdo.n;
+    const T* op = static_cast<const T*>(a.o) + b * a.so.b + hq * a.so.h + (int64_t)pos * a.so.n;
     Frag<T> of[KC];
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
@@ -52,11 +53,17 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(AttnArgs a) {
       of[c] = load_frag(op + d, a.D - d);
     }
     delta = row_dots<T, KC>(of, go);
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      arrive(q[c]);
+      arrive(go[c]);
+    }
   }
   const int64_t stat = ((int64_t)b * a.Hkv * a.grp + hq) * a.Nq + pos;
   // exponents' base; a row without a key has L = -inf: +inf here, so that every P is exp2(-inf) = 0
   float lse2 = a.lse[stat] * kLog2e;
   if (lse2 == -INFINITY) lse2 = INFINITY;
+  asm volatile("" : "+v"(lse2));   // here, not in the loop (arrive)
   if (sp == 0 && hi == 0 && row < a.R) a.delta[(int64_t)bh * a.R + row] = delta;
 
   const int lim = a.causal ? pos + a.off : a.Nk;
@@ -79,15 +86,22 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(AttnArgs a) {
   int t = 0;
   uint64_t live = 0;
   bool have = it.next(&t, &live);
-  TileLoad<T, DP, BN, NT> lk, lv;
+  TileLoad<T, DP, BN, NT, ODD> lk, lv;
   auto fetch = [&](int tile) {
-    lk.load(kp, a.D, [&](int n) { return (int64_t)min(tile * BN + n, a.Nk - 1) * a.sk.n; });
-    lv.load(vp, a.D, [&](int n) { return (int64_t)min(tile * BN + n, a.Nk - 1) * a.sv.n; });
+    const int last = a.Nk - 1 - tile * BN;
+    const T* k0 = kp + (int64_t)tile * BN * a.sk.n;
+    const T* v0 = vp + (int64_t)tile * BN * a.sv.n;
+    lk.load(a.D, [&](int n) { return k0 + (int64_t)min(n, last) * a.sk.n; });
+    lv.load(a.D, [&](int n) { return v0 + (int64_t)min(n, last) * a.sv.n; });
+  };
+  auto put = [&](int buf, uint64_t bits) {
+    lk.store(tk + buf * kTile, bits, a.D);
+    lv.store(tv + buf * kTile, bits, a.D);
+    if (threadIdx.x < BN) bias[buf * BN + threadIdx.x] = (bits >> threadIdx.x) & 1 ? 0.0f : -INFINITY;
   };
   if (have) {
     fetch(t);
-    lk.store(tk, live, a.D);
-    lv.store(tv, live, a.D);
+    put(0, live);
   }
   int buf = 0;
   while (have) {
@@ -99,22 +113,18 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(AttnArgs a) {
     const T* sk = tk + buf * kTile;
     const T* sv = tv + buf * kTile;
     const uint64_t all = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
-    const bool edge = live != all || t * BN + BN - 1 > lim0;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      Acc s = {}, p = {};
+      Acc s = live == all ? Acc{} : acc_rows(bias + buf * BN + kb * 32), p = {};
 #pragma unroll
       for (int c = 0; c < KC; ++c) s = mma(tile_frag<T, DP>(sk, kb * 32, c * 16), q[c], s);
 #pragma unroll
       for (int c = 0; c < KC; ++c) p = mma(tile_frag<T, DP>(sv, kb * 32, c * 16), go[c], p);
-      if (edge) {
-        const uint64_t lv64 = live >> (4 * hi);
+      if (t * BN + BN - 1 > lim0) {
         const int left = lim - t * BN - 4 * hi;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int k = kb * 32 + 8 * (i >> 2) + (i & 3);
-          if (!((lv64 >> k) & 1) || k > left) s[i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; ++i)
+          if (kb * 32 + 8 * (i >> 2) + (i & 3) > left) s[i] = -INFINITY;
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -127,10 +137,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(AttnArgs a) {
           dq[d] = mma(transpose_frag<T, DP>(sk, kb * 32 + c * 16, d * 32), ds, dq[d]);
       }
     }
-    if (more) {
-      lk.store(tk + (buf ^ 1) * kTile, ln, a.D);
-      lv.store(tv + (buf ^ 1) * kTile, ln, a.D);
-    }
+    if (more) put(buf ^ 1, ln);
     buf ^= 1;
     t = tn;
     live = ln;
@@ -139,7 +146,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(AttnArgs a) {
   if (row >= a.R) return;
   if (a.nsplit == 1) {
     if (!a.dq) return;
-    T* op = static_cast<T*>(a.dq) + b * a.sdq.b + hq * a.sdq.h + pos * a.sdq.n;
+    T* op = static_cast<T*>(a.dq) + b * a.sdq.b + hq * a.sdq.h + (int64_t)pos * a.sdq.n;
 #pragma unroll
     for (int d = 0; d < DB; ++d) store_column(op, a.D, d, dq[d], a.scale);
   } else {
@@ -159,7 +166,7 @@ __global__ __launch_bounds__(256) void k_attn_dq_join(AttnArgs a, int BH, int L)
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   int pos, h;
   attn_row(a, row, &pos, &h);
-  T* op = static_cast<T*>(a.dq) + b * a.sdq.b + (hk * a.grp + h) * a.sdq.h + pos * a.sdq.n;
+  T* op = static_cast<T*>(a.dq) + b * a.sdq.b + (hk * a.grp + h) * a.sdq.h + (int64_t)pos * a.sdq.n;
   for (int c = lig * 4; c < a.D; c += L * 4) {
     float x[4] = {};
 #pragma unroll 4
@@ -173,10 +180,10 @@ __global__ __launch_bounds__(256) void k_attn_dq_join(AttnArgs a, int BH, int L)
   }
 }
 
-template <typename T, int DP, int NW, int BN>
+template <typename T, int DP, int NW, int BN, bool ODD>
 int launch_dq(const AttnArgs& a, int blocks, hipStream_t stream) {
   static LdsLimit lim;
-  return launch_lds(k_attn_dq<T, DP, NW, BN>, lim, blocks, 64 * NW, dq_lds<T, DP, BN>(), a, stream);
+  return launch_lds(k_attn_dq<T, DP, NW, BN, ODD>, lim, blocks, 64 * NW, dq_lds<T, DP, BN>(), a, stream);
 }
 
 int attn_launch_dq(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hipStream_t stream) {
@@ -185,9 +192,10 @@ int attn_launch_dq(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hip
   const int blocks = p.rb_q * p.qs * BH;
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const int e = by_head(a.D, [&](auto dp) {
-      if (p.qw == 1) return launch_dq<T, dp(), 1, 32>(a, blocks, stream);
-      return launch_dq<T, dp(), 4, 64>(a, blocks, stream);
+    const int e = by_head(a.D, [&](auto dp, auto odd) {
+      if constexpr (!odd())
+        if (p.qw == 1) return launch_dq<T, dp(), 1, 32, false>(a, blocks, stream);
+      return launch_dq<T, dp(), 4, 64, odd()>(a, blocks, stream);
     });
     if (e || p.qs == 1 || !a.dq) return e;
     const int L = row_lanes((a.D + 3) / 4);

@@ -17,16 +17,17 @@ namespace tts {
 
 template <typename T, int DP, int BN>
 constexpr size_t fwd_lds() {
-  return (size_t)4 * BN * kTileStride<T, DP> * sizeof(T);
+  return (size_t)4 * BN * kTileStride<T, DP> * sizeof(T) + 2 * BN * sizeof(float);
 }
 
-template <typename T, int DP, int NW, int BN>
-__global__ __launch_bounds__(64 * NW) void k_attn_fwd(AttnArgs a) {
+template <typename T, int DP, int NW, int BN, bool ODD>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2 : 1) void k_attn_fwd(AttnArgs a) {
   constexpr int KC = DP / 16, DB = DP / 32, KB = BN / 32, NT = 64 * NW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* tk = reinterpret_cast<T*>(smem);
   constexpr int kTile = BN * kTileStride<T, DP>;
   T* tv = tk + 2 * kTile;
+  float* bias = reinterpret_cast<float*>(tv + 2 * kTile);   // [2][BN] 0, or -inf for hidden keys
 
   const int nrb = (a.R + 32 * NW - 1) / (32 * NW);
   const int item = xcd_item(blockIdx.x, gridDim.x);
@@ -45,6 +46,8 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(AttnArgs a) {
                   row_offset(a.sq, pos, h);
 #pragma unroll
     for (int c = 0; c < KC; ++c) q[c] = load_frag(qp + c * 16 + hi * 8, a.D - c * 16 - hi * 8);
+#pragma unroll
+    for (int c = 0; c < KC; ++c) arrive(q[c]);
   }
   const int lim = a.causal ? pos + a.off : a.Nk;   // the row sees keys up to lim
   // keys that any row of the block sees
@@ -73,15 +76,22 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(AttnArgs a) {
   int t = 0;
   uint64_t live = 0;
   bool have = it.next(&t, &live);
-  TileLoad<T, DP, BN, NT> lk, lv;
+  TileLoad<T, DP, BN, NT, ODD> lk, lv;
   auto fetch = [&](int tile) {
-    lk.load(kp, a.D, [&](int n) { return (int64_t)min(tile * BN + n, a.Nk - 1) * a.sk.n; });
-    lv.load(vp, a.D, [&](int n) { return (int64_t)min(tile * BN + n, a.Nk - 1) * a.sv.n; });
+    const int last = a.Nk - 1 - tile * BN;
+    const T* k0 = kp + (int64_t)tile * BN * a.sk.n;
+    const T* v0 = vp + (int64_t)tile * BN * a.sv.n;
+    lk.load(a.D, [&](int n) { return k0 + (int64_t)min(n, last) * a.sk.n; });
+    lv.load(a.D, [&](int n) { return v0 + (int64_t)min(n, last) * a.sv.n; });
+  };
+  auto put = [&](int buf, uint64_t bits) {
+    lk.store(tk + buf * kTile, bits, a.D);
+    lv.store(tv + buf * kTile, bits, a.D);
+    if (threadIdx.x < BN) bias[buf * BN + threadIdx.x] = (bits >> threadIdx.x) & 1 ? 0.0f : -INFINITY;
   };
   if (have) {
     fetch(t);
-    lk.store(tk, live, a.D);
-    lv.store(tv, live, a.D);
+    put(0, live);
   }
   int buf = 0;
   while (have) {
@@ -93,23 +103,22 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(AttnArgs a) {
     const T* sk = tk + buf * kTile;
     const T* sv = tv + buf * kTile;
 
-    Acc s[KB] = {};
+    const uint64_t all = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
+    Acc s[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) s[kb] = live == all ? Acc{} : acc_rows(bias + buf * BN + kb * 32);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int c = 0; c < KC; ++c) s[kb] = mma(tile_frag<T, DP>(sk, kb * 32, c * 16), q[c], s[kb]);
 
-    const uint64_t all = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
-    if (live != all || t * BN + BN - 1 > lim0) {
-      const uint64_t lv64 = live >> (4 * hi);
+    if (t * BN + BN - 1 > lim0) {
       const int left = lim - t * BN - 4 * hi;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int k = kb * 32 + 8 * (i >> 2) + (i & 3);
-          if (!((lv64 >> k) & 1) || k > left) s[kb][i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; ++i)
+          if (kb * 32 + 8 * (i >> 2) + (i & 3) > left) s[kb][i] = -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
@@ -146,10 +155,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(AttnArgs a) {
           o[d] = mma(transpose_frag<T, DP>(sv, kb * 32 + c * 16, d * 32), p, o[d]);
       }
     }
-    if (more) {
-      lk.store(tk + (buf ^ 1) * kTile, ln, a.D);
-      lv.store(tv + (buf ^ 1) * kTile, ln, a.D);
-    }
+    if (more) put(buf ^ 1, ln);
     buf ^= 1;
     t = tn;
     live = ln;
@@ -162,7 +168,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(AttnArgs a) {
   if (row >= a.R) return;
   if (a.nsplit == 1) {
     const int hq = hk * a.grp + h;
-    T* op = static_cast<T*>(a.out) + b * a.so.b + hq * a.so.h + pos * a.so.n;
+    T* op = static_cast<T*>(a.out) + b * a.so.b + hq * a.so.h + (int64_t)pos * a.so.n;
 #pragma unroll
     for (int d = 0; d < DB; ++d) store_column(op, a.D, d, o[d], inv);
     if (a.lse && hi == 0) a.lse[((int64_t)b * a.Hkv * a.grp + hq) * a.Nq + pos] = lse;
@@ -191,7 +197,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int BH, int L) {
   // a NaN in any part reaches the sum, as it does in one pass
   for (int s = 0; s < a.nsplit; ++s) l += exp2_((a.part2[s * rows + i] - base) * kLog2e);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  T* op = static_cast<T*>(a.out) + b * a.so.b + hq * a.so.h + pos * a.so.n;
+  T* op = static_cast<T*>(a.out) + b * a.so.b + hq * a.so.h + (int64_t)pos * a.so.n;
   for (int c = lig * 4; c < a.D; c += L * 4) {
     float x[4] = {};
 #pragma unroll 4
@@ -209,10 +215,10 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int BH, int L) {
         l == 0.0f ? -INFINITY : base + kLn2 * __log2f(l);
 }
 
-template <typename T, int DP, int NW, int BN>
+template <typename T, int DP, int NW, int BN, bool ODD>
 int launch_fwd(const AttnArgs& a, int blocks, hipStream_t stream) {
   static LdsLimit lim;
-  return launch_lds(k_attn_fwd<T, DP, NW, BN>, lim, blocks, 64 * NW, fwd_lds<T, DP, BN>(), a,
+  return launch_lds(k_attn_fwd<T, DP, NW, BN, ODD>, lim, blocks, 64 * NW, fwd_lds<T, DP, BN>(), a,
                     stream);
 }
 
@@ -222,9 +228,10 @@ int attn_launch_fwd(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hi
   const int blocks = p.rb_f * p.fs * BH;
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const int e = by_head(a.D, [&](auto dp) {
-      if (p.fw == 1) return launch_fwd<T, dp(), 1, 32>(a, blocks, stream);
-      return launch_fwd<T, dp(), 4, 64>(a, blocks, stream);
+    const int e = by_head(a.D, [&](auto dp, auto odd) {
+      if constexpr (!odd())
+        if (p.fw == 1) return launch_fwd<T, dp(), 1, 32, false>(a, blocks, stream);
+      return launch_fwd<T, dp(), 4, 64, odd()>(a, blocks, stream);
     });
     if (e || p.fs == 1) return e;
     const int L = row_lanes((a.D + 3) / 4);
