@@ -56,7 +56,7 @@ extern "C" {
 #define TTS_ESH (-8)        /* SH degree outside [0, 3], or rest coefficients missing */
 #define TTS_ESCRATCH (-9)   /* sizes beyond the fixed scratch of an allocation-free entry point */
 #define TTS_EDTYPE (-10)    /* element type not TTS_F32/F16/BF16, or weights of a third type */
-#define TTS_ELENGTH (-11)   /* a length over an entry's limit */
+#define TTS_ELENGTH (-11)   /* a length or a row stride over an entry's limit */
 #define TTS_EHEADS (-12)    /* head size outside [1, 128], or heads not a multiple of kv_heads */
 
 /* Library version, (major << 16) | minor. */
@@ -651,7 +651,7 @@ int tts_embedding_bwd(const void* dout, const void* ids, int ids64, int64_t N, i
                       size_t workspace_bytes, hipStream_t stream);
 
 /* Shape of an attention call.  Strides are in elements, of (batch, head, row); the head_dim values of a
- * row are contiguous; any alignment of the element.  heads is a multiple of kv_heads: query head h
+ * row are contiguous; any alignment of the element; a row's stride is below 2^23.  heads is a multiple of kv_heads: query head h
  * reads key head h / (heads / kv_heads).  The strides o are of out; dout, dq, dk and dv are read by the
  * backward alone. */
 typedef struct tts_attention_shape {

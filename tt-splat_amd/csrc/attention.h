@@ -46,7 +46,8 @@ __device__ __forceinline__ Acc mma(Frag<float> a, Frag<float> b, Acc c) {
   return c;
 }
 
-// Strides in elements of (batch, head, row); a row's is below 2^31, its product with a row is 64-bit.
+// Strides in elements of (batch, head, row).  A row's is below 2^23: a tile's rows are then within 2^31
+// bytes of its first; products with a row of the whole axis are 64-bit.
 struct AttnStride {
   int64_t b, h;
   int n;
@@ -60,20 +61,18 @@ struct AttnArgs {
   int64_t mask_stride;
   AttnStride sq, sk, sv, so, sdo, sdq, sdk, sdv;
   int Hkv, grp, Nq, Nk, D, R;   // R = Nq * grp rows a (batch, key head)
+  unsigned grp_mul;             // r / grp = (4 r * grp_mul >> 32) >> grp_shift for r < 2^30
+  int grp_shift;
   int causal, off;              // row at position p sees keys up to p + off
   int nsplit;                   // parts of the long axis, joined by a second kernel
   float scale;
 };
 
-// Position and head of a row.
+// Position and head of a row.  grp_mul = ceil(2^(30 + grp_shift) / grp), 2^grp_shift >= grp: the product
+// is too large by less than r 2^grp_shift < 2^(30 + grp_shift), less than one in the quotient.
 __device__ __forceinline__ void attn_row(const AttnArgs& a, int r, int* pos, int* h) {
-  if (a.grp == 1) {
-    *pos = r;
-    *h = 0;
-  } else {
-    *pos = (int)((unsigned)r / (unsigned)a.grp);
-    *h = r - *pos * a.grp;
-  }
+  *pos = (int)(__umulhi((unsigned)r << 2, a.grp_mul) >> a.grp_shift);
+  *h = r - *pos * a.grp;
 }
 __device__ __forceinline__ int64_t row_offset(const AttnStride& s, int pos, int h) {
   return h * s.h + (int64_t)pos * s.n;
@@ -105,10 +104,12 @@ __device__ __forceinline__ void arrive(F& f) {
   memcpy(&f, v, sizeof(F));
 }
 
-// Tiles in LDS: row-major, rows 16 bytes longer than their data, which spreads the rows of one
-// fragment (32 lanes, 16 bytes each) and of one transposed read over the banks.
+// Tiles in LDS: row-major, rows longer than their data so that one read's lanes meet different banks
+// (64 of 4 bytes).  Half types: 32 bytes longer, a stride of 8 banks past a multiple of 16; a fragment's
+// 8 lanes a clock take 4 banks each of 8 rows, a transposed read's 16 lanes 8 banks each of 4 rows.
+// fp32: 16 bytes longer; transposed reads take 32 values of one row.
 template <typename T, int DP>
-constexpr int kTileStride = DP + 16 / (int)sizeof(T);
+constexpr int kTileStride = DP + (sizeof(T) == 2 ? 16 : 4);
 
 template <typename T, int DP>
 __device__ __forceinline__ Frag<T> tile_frag(const T* tile, int row0, int d0) {
@@ -149,7 +150,7 @@ __device__ __forceinline__ Frag<T> transpose_frag(const T* tile, int row0, int d
 // writes the tile, zeros for rows not in `live` (masked and missing keys: whatever stands there, NaN
 // among it, stays out of the products) and past the head size.  ODD: head sizes that are no multiple
 // of eight, read value by value; a branch for them in the same kernel makes the compiler wait for
-// the loads at once, which costs the overlap (2500 x 2500 bf16 forward 95 -> TODO us).
+// the loads at once, which costs the overlap (2500 x 2500 bf16 forward 95 -> 80 us).
 template <typename T, int DP, int BN, int NT, bool ODD>
 struct TileLoad {
   static constexpr int kPerRow = DP / 8, kN = BN * kPerRow / NT;
@@ -162,25 +163,60 @@ struct TileLoad {
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int v = threadIdx.x + i * NT, d0 = v % kPerRow * 8;
-      const T* p = row(v / kPerRow);
-      if constexpr (ODD) {
+      get(i, row(v / kPerRow), d0, D);
+    }
+  }
+  // rows `first` (uniform) + min(n, last) * stride, 32-bit offsets from the first
+  __device__ __forceinline__ void load_rows(int D, const T* first, int stride, int last) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r[i][j] = p[d0 + j < D ? d0 + j : 0];
+    for (int i = 0; i < kN; ++i) {
+      const int v = threadIdx.x + i * NT, d0 = v % kPerRow * 8, n = min(v / kPerRow, last);
+      if constexpr (ODD) {
+        get(i, first + n * stride, d0, D);
       } else {
-        memcpy(&r[i], p + (d0 < D ? d0 : 0), 8 * sizeof(T));
+        const unsigned off = (unsigned)(n * stride + (d0 < D ? d0 : 0)) * (unsigned)sizeof(T);
+        memcpy(&r[i], reinterpret_cast<const char*>(first) + off, 8 * sizeof(T));
       }
     }
   }
+  __device__ __forceinline__ void get(int i, const T* p, int d0, int D) {
+    if constexpr (ODD) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[i][j] = p[d0 + j < D ? d0 + j : 0];
+    } else {
+      memcpy(&r[i], p + (d0 < D ? d0 : 0), 8 * sizeof(T));
+    }
+  }
   __device__ __forceinline__ void store(T* tile, uint64_t live, int D) const {
+    constexpr int kWords = 2 * (int)sizeof(T);
+    if (!ODD && D == DP && live == (BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1)) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int v = threadIdx.x + i * NT;
+        memcpy(at(tile, v), &r[i], 8 * sizeof(T));
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int v = threadIdx.x + i * NT, n = v / kPerRow, d0 = v % kPerRow * 8;
-      const bool on = ((live >> n) & 1) && d0 < D;
+      const uint32_t bits = n < 32 ? (uint32_t)live : (uint32_t)(live >> 32);
+      const bool on = (bits >> (n & 31) & 1) && d0 < D;
       Frag<T> f = r[i];
+      if constexpr (ODD) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = on && (!ODD || d0 + j < D) ? f[j] : (T)0.0f;
-      memcpy(__builtin_assume_aligned(tile + n * kTileStride<T, DP> + d0, 16), &f, 8 * sizeof(T));
+        for (int j = 0; j < 8; ++j) f[j] = d0 + j < D ? f[j] : (T)0.0f;
+      }
+      uint32_t w[kWords];
+      memcpy(w, &f, sizeof(f));
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) w[j] = on ? w[j] : 0;
+      memcpy(at(tile, v), w, sizeof(f));
     }
+  }
+  static __device__ __forceinline__ T* at(T* tile, int v) {
+    return static_cast<T*>(__builtin_assume_aligned(
+        tile + v / kPerRow * kTileStride<T, DP> + v % kPerRow * 8, 16));
   }
 };
 
@@ -365,7 +401,7 @@ inline int attn_splits(int64_t blocks, int tiles, int least) {
 
 // Blocks and splits of each kernel for a shape.
 struct AttnPlan {
-  int fw, fs;        // forward: waves a block, splits
+  int fw, fs, fq;    // forward: waves a block, splits, blocks of 32 rows a wave
   int qw, qs;        // dq
   int kw, ks;        // dk, dv
   int rb_f, rb_q, kb;

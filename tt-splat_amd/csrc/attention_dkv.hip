@@ -10,6 +10,7 @@
 // k_attn_dkv_join adds the parts in order.
 
 #include "attention.h"
+#include <cstdlib>
 
 namespace tts {
 
@@ -20,7 +21,7 @@ constexpr size_t dkv_lds() {
   return (size_t)4 * BM * kTileStride<T, DP> * sizeof(T) + 2 * 3 * BM * sizeof(float);
 }
 
-template <typename T, int DP, int NW, int BM, bool ODD>
+template <typename T, int DP, int NW, int BM, bool ODD, bool CAUSAL>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
   constexpr int KC = DP / 16, DB = DP / 32, NT = 64 * NW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -65,7 +66,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void k
   const int tiles = (a.R + BM - 1) / BM;
   int t = (int)((int64_t)tiles * sp / a.nsplit);
   int t1 = (int)((int64_t)tiles * (sp + 1) / a.nsplit);
-  if (a.causal) {
+  if constexpr (CAUSAL) {
     const int64_t first = (int64_t)max(key0 - a.off, 0) * a.grp / BM;
     t = (int)(first > t ? (first < t1 ? first : t1) : t);
   }
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void k
         for (int c = 0; c < KC; ++c) s = mma(tile_frag<T, DP>(sq, rb, c * 16), k[c], s);
 #pragma unroll
         for (int c = 0; c < KC; ++c) p = mma(tile_frag<T, DP>(sg, rb, c * 16), v[c], p);
-        if (a.causal) {
+        if constexpr (CAUSAL) {
           const Acc lim = acc_rows(st + 2 * BM + rb);
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -217,9 +218,12 @@ __global__ __launch_bounds__(256) void k_attn_dkv_join(AttnArgs a, int BH, int L
 
 template <typename T, int DP, int NW, int BM, bool ODD>
 int launch_dkv(const AttnArgs& a, int blocks, hipStream_t stream) {
-  static LdsLimit lim;
-  return launch_lds(k_attn_dkv<T, DP, NW, BM, ODD>, lim, blocks, 64 * NW, dkv_lds<T, DP, BM>(), a,
-                    stream);
+  static LdsLimit lim, lim_causal;
+  constexpr size_t lds = dkv_lds<T, DP, BM>();
+  if (a.causal)
+    return launch_lds(k_attn_dkv<T, DP, NW, BM, ODD, true>, lim_causal, blocks, 64 * NW, lds, a,
+                      stream);
+  return launch_lds(k_attn_dkv<T, DP, NW, BM, ODD, false>, lim, blocks, 64 * NW, lds, a, stream);
 }
 
 int attn_launch_dkv(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hipStream_t stream) {
@@ -247,11 +251,15 @@ AttnPlan attn_plan(const AttnArgs& a, int BH) {
   AttnPlan p;
   p.fw = p.qw = a.R <= 32 && a.D % 8 == 0 ? 1 : 4;
   const int bn = p.fw == 1 ? 32 : 64, tiles = (a.Nk - 1) / bn + 1;
-  p.rb_f = p.rb_q = (a.R - 1) / (32 * p.fw) + 1;
+  p.fq = getenv("FQ2") && p.fw == 4 ? 2 : 1;
+  p.rb_q = (a.R - 1) / (32 * p.fw) + 1;
+  p.rb_f = (a.R - 1) / (32 * p.fw * p.fq) + 1;
   p.fs = p.qs = attn_splits((int64_t)p.rb_f * BH, tiles, p.fw == 1 ? 2 : 4);
   p.kw = a.Nk <= 32 && a.D % 8 == 0 ? 1 : 4;
   p.kb = (a.Nk - 1) / (32 * p.kw) + 1;
   p.ks = attn_splits((int64_t)p.kb * BH, (a.R - 1) / (p.kw == 1 ? 32 : kDkvRows) + 1, 2);
+  auto ev = [](const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; };
+  p.fs = ev("FS", p.fs); p.qs = ev("QS", p.qs); p.ks = ev("KS", p.ks);
   return p;
 }
 
@@ -289,7 +297,7 @@ int attn_shape(const tts_attention_shape* s, AttnArgs* a, int* BH) {
     return TTS_ELENGTH;
   *a = AttnArgs{};
   for (const int64_t* x : {s->q, s->k, s->v, s->o, s->dout, s->dq, s->dk, s->dv})
-    if (x[2] < 0 || x[2] >= (int64_t)1 << 31) return TTS_ELENGTH;
+    if (x[2] < 0 || x[2] >= (int64_t)1 << 23) return TTS_ELENGTH;
   auto st = [](const int64_t* x) { return AttnStride{x[0], x[1], (int)x[2]}; };
   a->sq = st(s->q);
   a->sk = st(s->k);
@@ -306,6 +314,8 @@ int attn_shape(const tts_attention_shape* s, AttnArgs* a, int* BH) {
   a->Nk = (int)s->keys;
   a->D = (int)s->head_dim;
   a->R = (int)(s->queries * grp);
+  while ((1 << a->grp_shift) < grp) ++a->grp_shift;
+  a->grp_mul = (unsigned)((((uint64_t)1 << (30 + a->grp_shift)) + grp - 1) / grp);
   a->causal = s->causal != 0;
   a->off = (int)(s->keys - s->queries);
   a->scale = (float)s->scale;

@@ -67,14 +67,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
   if (sp == 0 && hi == 0 && row < a.R) a.delta[(int64_t)bh * a.R + row] = delta;
 
   const int lim = a.causal ? pos + a.off : a.Nk;
-  int nk = a.Nk, lim0 = a.Nk;
+  const int lim0 = __builtin_amdgcn_readfirstlane(lim);   // seen by every row of the wave
+  int nk = a.Nk;
   if (a.causal) {
     int p1, h1;
     const int last = (rb + 1) * NW * 32 - 1;
     attn_row(a, last < a.R ? last : a.R - 1, &p1, &h1);
     nk = min(nk, max(p1 + a.off + 1, 0));
-    attn_row(a, row0 < a.R ? row0 : a.R - 1, &p1, &h1);
-    lim0 = p1 + a.off;
   }
   const int tiles = (a.Nk + BN - 1) / BN, need = (nk + BN - 1) / BN;
   const int t0 = (int)((int64_t)tiles * sp / a.nsplit), t1 = (int)((int64_t)tiles * (sp + 1) / a.nsplit);
@@ -91,8 +90,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
     const int last = a.Nk - 1 - tile * BN;
     const T* k0 = kp + (int64_t)tile * BN * a.sk.n;
     const T* v0 = vp + (int64_t)tile * BN * a.sv.n;
-    lk.load(a.D, [&](int n) { return k0 + (int64_t)min(n, last) * a.sk.n; });
-    lv.load(a.D, [&](int n) { return v0 + (int64_t)min(n, last) * a.sv.n; });
+    lk.load_rows(a.D, k0, a.sk.n, last);
+    lv.load_rows(a.D, v0, a.sv.n, last);
   };
   auto put = [&](int buf, uint64_t bits) {
     lk.store(tk + buf * kTile, bits, a.D);
@@ -121,7 +120,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
 #pragma unroll
       for (int c = 0; c < KC; ++c) p = mma(tile_frag<T, DP>(sv, kb * 32, c * 16), go[c], p);
       if (t * BN + BN - 1 > lim0) {
-        const int left = lim - t * BN - 4 * hi;
+        int left = lim - t * BN - 4 * hi;
+        asm volatile("" : "+v"(left));   // made here: a branch, not selects in every tile
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (kb * 32 + 8 * (i >> 2) + (i & 3) > left) s[i] = -INFINITY;

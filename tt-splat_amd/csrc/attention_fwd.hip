@@ -20,8 +20,9 @@ constexpr size_t fwd_lds() {
   return (size_t)4 * BN * kTileStride<T, DP> * sizeof(T) + 2 * BN * sizeof(float);
 }
 
-template <typename T, int DP, int NW, int BN, bool ODD>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2 : 1) void k_attn_fwd(AttnArgs a) {
+template <typename T, int DP, int NW, int BN, int QB, bool ODD>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) && QB * DP <= 128 ? 2 : 1)
+void k_attn_fwd(AttnArgs a) {
   constexpr int KC = DP / 16, DB = DP / 32, KB = BN / 32, NT = 64 * NW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* tk = reinterpret_cast<T*>(smem);
@@ -29,7 +30,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
   T* tv = tk + 2 * kTile;
   float* bias = reinterpret_cast<float*>(tv + 2 * kTile);   // [2][BN] 0, or -inf for hidden keys
 
-  const int nrb = (a.R + 32 * NW - 1) / (32 * NW);
+  constexpr int kRows = 32 * QB * NW;
+  const int nrb = (a.R + kRows - 1) / kRows;
   const int item = xcd_item(blockIdx.x, gridDim.x);
   const int rb = item % nrb, sp = item / nrb % a.nsplit, bh = item / nrb / a.nsplit;
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
@@ -37,38 +39,42 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
   const T* kp = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
   const T* vp = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
 
-  const int row0 = (rb * NW + wave) * 32, row = row0 + (lane & 31);
-  int pos, h;
-  attn_row(a, row < a.R ? row : a.R - 1, &pos, &h);
-  Frag<T> q[KC];
-  {
+  const int row0 = (rb * NW + wave) * 32 * QB + (lane & 31);   // the lane's rows: row0 + 32 j
+  Frag<T> q[QB][KC];
+  int lim[QB];   // the row sees keys up to lim
+#pragma unroll
+  for (int j = 0; j < QB; ++j) {
+    int pos, h;
+    attn_row(a, min(row0 + 32 * j, a.R - 1), &pos, &h);
     const T* qp = static_cast<const T*>(a.q) + b * a.sq.b + (int64_t)hk * a.grp * a.sq.h +
                   row_offset(a.sq, pos, h);
 #pragma unroll
-    for (int c = 0; c < KC; ++c) q[c] = load_frag(qp + c * 16 + hi * 8, a.D - c * 16 - hi * 8);
-#pragma unroll
-    for (int c = 0; c < KC; ++c) arrive(q[c]);
+    for (int c = 0; c < KC; ++c) q[j][c] = load_frag(qp + c * 16 + hi * 8, a.D - c * 16 - hi * 8);
+    lim[j] = a.causal ? pos + a.off : a.Nk;
   }
-  const int lim = a.causal ? pos + a.off : a.Nk;   // the row sees keys up to lim
+#pragma unroll
+  for (int j = 0; j < QB; ++j)
+#pragma unroll
+    for (int c = 0; c < KC; ++c) arrive(q[j][c]);
   // keys that any row of the block sees
   int nk = a.Nk;
   if (a.causal) {
     int p1, h1;
-    const int last = (rb + 1) * NW * 32 - 1;
-    attn_row(a, last < a.R ? last : a.R - 1, &p1, &h1);
+    attn_row(a, min((rb + 1) * kRows - 1, a.R - 1), &p1, &h1);
     nk = min(nk, max(p1 + a.off + 1, 0));
   }
-  int lim0 = a.Nk;   // keys up to lim0 are seen by every row of the wave
-  if (a.causal) {
-    int p0, h0;
-    attn_row(a, row0 < a.R ? row0 : a.R - 1, &p0, &h0);
-    lim0 = p0 + a.off;
-  }
+  // keys up to lim0 are seen by every row of the wave: its first row's, the same in all lanes
+  const int lim0 = __builtin_amdgcn_readfirstlane(lim[0]);
   const int tiles = (a.Nk + BN - 1) / BN, need = (nk + BN - 1) / BN;
   const int t0 = (int)((int64_t)tiles * sp / a.nsplit), t1 = (int)((int64_t)tiles * (sp + 1) / a.nsplit);
 
-  Acc o[DB] = {};
-  float m = -INFINITY, l = 0.0f;
+  Acc o[QB][DB] = {};
+  float m[QB], l[QB];
+#pragma unroll
+  for (int j = 0; j < QB; ++j) {
+    m[j] = -INFINITY;
+    l[j] = 0.0f;
+  }
   const float c2 = a.scale * kLog2e;
 
   KeyTiles<BN> it;
@@ -81,8 +87,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
     const int last = a.Nk - 1 - tile * BN;
     const T* k0 = kp + (int64_t)tile * BN * a.sk.n;
     const T* v0 = vp + (int64_t)tile * BN * a.sv.n;
-    lk.load(a.D, [&](int n) { return k0 + (int64_t)min(n, last) * a.sk.n; });
-    lv.load(a.D, [&](int n) { return v0 + (int64_t)min(n, last) * a.sv.n; });
+    lk.load_rows(a.D, k0, a.sk.n, last);
+    lv.load_rows(a.D, v0, a.sv.n, last);
   };
   auto put = [&](int buf, uint64_t bits) {
     lk.store(tk + buf * kTile, bits, a.D);
@@ -104,55 +110,80 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
     const T* sv = tv + buf * kTile;
 
     const uint64_t all = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
-    Acc s[KB];
+    Acc s[KB][QB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) s[kb] = live == all ? Acc{} : acc_rows(bias + buf * BN + kb * 32);
+    for (int kb = 0; kb < KB; ++kb) {
+      const Acc z = live == all ? Acc{} : acc_rows(bias + buf * BN + kb * 32);
+#pragma unroll
+      for (int j = 0; j < QB; ++j) s[kb][j] = z;
+    }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int c = 0; c < KC; ++c) s[kb] = mma(tile_frag<T, DP>(sk, kb * 32, c * 16), q[c], s[kb]);
+      for (int c = 0; c < KC; ++c) {
+        const Frag<T> f = tile_frag<T, DP>(sk, kb * 32, c * 16);
+#pragma unroll
+        for (int j = 0; j < QB; ++j) s[kb][j] = mma(f, q[j][c], s[kb][j]);
+      }
 
     if (t * BN + BN - 1 > lim0) {
-      const int left = lim - t * BN - 4 * hi;
+#pragma unroll
+      for (int j = 0; j < QB; ++j) {
+        int left = lim[j] - t * BN - 4 * hi;
+        asm volatile("" : "+v"(left));   // made here: a branch, not selects in every tile
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (kb * 32 + 8 * (i >> 2) + (i & 3) > left) s[kb][j][i] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < QB; ++j) {
+      float mx = s[0][j][0];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (kb * 32 + 8 * (i >> 2) + (i & 3) > left) s[kb][i] = -INFINITY;
-    }
-    float mx = s[0][0];
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][j][i]);
+      mx = fmaxf(m[j], max_halves(mx));
+      // The exponents' base follows the maximum where it lags by more than 2^8: P up to 256 is as exact
+      // as P up to 1, and past a row's first tile O is hardly ever scaled.
+      if (__ballot((mx - m[j]) * c2 > 8.0f)) {
+        const float f = mx == -INFINITY ? 1.0f : exp2_((m[j] - mx) * c2);
+        l[j] *= f;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-    mx = fmaxf(m, max_halves(mx));
-    // a row without a key so far keeps -inf and takes 0 for its exponents' base: exp2(-inf) = 0
-    const float top = mx == -INFINITY ? 0.0f : mx, base = top * c2;
-    if (__ballot(mx > m)) {
-      const float f = exp2_((m - top) * c2);
-      l *= f;
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] *= f;
-      m = mx;
+          for (int i = 0; i < 16; ++i) o[j][d][i] *= f;
+        m[j] = mx;
+      }
     }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        // fp32: exactly 1 at the maximum, so that a row with one key gives its v to the last bit;
-        // half types round P to fewer bits than the one operation less can lose
-        s[kb][i] = sizeof(T) == 4 ? exp2_((s[kb][i] - top) * c2)
-                                  : exp2_(__builtin_fmaf(s[kb][i], c2, -base));
-        l += s[kb][i];
+      for (int j = 0; j < QB; ++j) {
+        // a row without a key so far keeps -inf and takes 0 for its base: exp2(-inf) = 0
+        const float top = m[j] == -INFINITY ? 0.0f : m[j], base = top * c2;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          // fp32: exactly 1 at the maximum, so that a row with one key gives its v to the last bit;
+          // half types round P to fewer bits than the one operation less can lose
+          s[kb][j][i] = sizeof(T) == 4 ? exp2_((s[kb][j][i] - top) * c2)
+                                       : exp2_(__builtin_fmaf(s[kb][j][i], c2, -base));
+          l[j] += s[kb][j][i];
+        }
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const Frag<T> p = acc_frag<T>(s[kb], c);
+        Frag<T> p[QB];
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-          o[d] = mma(transpose_frag<T, DP>(sv, kb * 32 + c * 16, d * 32), p, o[d]);
+        for (int j = 0; j < QB; ++j) p[j] = acc_frag<T>(s[kb][j], c);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const Frag<T> f = transpose_frag<T, DP>(sv, kb * 32 + c * 16, d * 32);
+#pragma unroll
+          for (int j = 0; j < QB; ++j) o[j][d] = mma(f, p[j], o[j][d]);
+        }
       }
     }
     if (more) put(buf ^ 1, ln);
@@ -162,21 +193,27 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
     have = more;
   }
 
-  l = sum_halves(l);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const float lse = l == 0.0f ? -INFINITY : m * a.scale + kLn2 * __log2f(l);
-  if (row >= a.R) return;
-  if (a.nsplit == 1) {
-    const int hq = hk * a.grp + h;
-    T* op = static_cast<T*>(a.out) + b * a.so.b + hq * a.so.h + (int64_t)pos * a.so.n;
 #pragma unroll
-    for (int d = 0; d < DB; ++d) store_column(op, a.D, d, o[d], inv);
-    if (a.lse && hi == 0) a.lse[((int64_t)b * a.Hkv * a.grp + hq) * a.Nq + pos] = lse;
-  } else {
-    const int64_t i = ((int64_t)sp * (gridDim.x / nrb / a.nsplit) + bh) * a.R + row;
+  for (int j = 0; j < QB; ++j) {
+    const int row = row0 + 32 * j;
+    const float sum = sum_halves(l[j]);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float lse = sum == 0.0f ? -INFINITY : m[j] * a.scale + kLn2 * __log2f(sum);
+    if (row >= a.R) continue;
+    if (a.nsplit == 1) {
+      int pos, h;
+      attn_row(a, row, &pos, &h);
+      const int hq = hk * a.grp + h;
+      T* op = static_cast<T*>(a.out) + b * a.so.b + hq * a.so.h + (int64_t)pos * a.so.n;
 #pragma unroll
-    for (int d = 0; d < DB; ++d) store_column(a.part + i * a.D, a.D, d, o[d], inv);
-    if (hi == 0) a.part2[i] = lse;
+      for (int d = 0; d < DB; ++d) store_column(op, a.D, d, o[j][d], inv);
+      if (a.lse && hi == 0) a.lse[((int64_t)b * a.Hkv * a.grp + hq) * a.Nq + pos] = lse;
+    } else {
+      const int64_t i = ((int64_t)sp * (gridDim.x / nrb / a.nsplit) + bh) * a.R + row;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) store_column(a.part + i * a.D, a.D, d, o[j][d], inv);
+      if (hi == 0) a.part2[i] = lse;
+    }
   }
 }
 
@@ -215,10 +252,10 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int BH, int L) {
         l == 0.0f ? -INFINITY : base + kLn2 * __log2f(l);
 }
 
-template <typename T, int DP, int NW, int BN, bool ODD>
+template <typename T, int DP, int NW, int BN, int QB, bool ODD>
 int launch_fwd(const AttnArgs& a, int blocks, hipStream_t stream) {
   static LdsLimit lim;
-  return launch_lds(k_attn_fwd<T, DP, NW, BN, ODD>, lim, blocks, 64 * NW, fwd_lds<T, DP, BN>(), a,
+  return launch_lds(k_attn_fwd<T, DP, NW, BN, QB, ODD>, lim, blocks, 64 * NW, fwd_lds<T, DP, BN>(), a,
                     stream);
 }
 
@@ -230,8 +267,10 @@ int attn_launch_fwd(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hi
     using T = decltype(t);
     const int e = by_head(a.D, [&](auto dp, auto odd) {
       if constexpr (!odd())
-        if (p.fw == 1) return launch_fwd<T, dp(), 1, 32, false>(a, blocks, stream);
-      return launch_fwd<T, dp(), 4, 64, odd()>(a, blocks, stream);
+        if (p.fw == 1) return launch_fwd<T, dp(), 1, 32, 1, false>(a, blocks, stream);
+      if constexpr (!odd() && sizeof(T) == 2)
+        if (p.fq == 2) return launch_fwd<T, dp(), 4, 64, 2, false>(a, blocks, stream);
+      return launch_fwd<T, dp(), 4, 64, 1, odd()>(a, blocks, stream);
     });
     if (e || p.fs == 1) return e;
     const int L = row_lanes((a.D + 3) / 4);

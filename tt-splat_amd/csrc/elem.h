@@ -4,6 +4,8 @@
 
 #include <string.h>
 
+#include <type_traits>
+
 #include "tts_common.h"
 
 namespace tts {
@@ -27,18 +29,82 @@ __device__ __forceinline__ Pack<T> load_pack(const T* p) {
   memcpy(&r, p, 16);
   return r;
 }
-// Elements [0, n) of the vector at p as floats, zeros behind them.  The last vector of a row is
-// read element by element: nothing past the row is touched.
+// How a row of `cols` values divides into vectors: evenly, with a tail, or shorter than one.
+enum RowMode { kRowEven, kRowTail, kRowTiny };
+template <typename T>
+inline RowMode row_mode(int cols) {
+  return cols % kVec<T> == 0 ? kRowEven : cols < kVec<T> ? kRowTiny : kRowTail;
+}
+// f(integral_constant) by the row's mode.
+template <typename T, typename F>
+inline int by_row_mode(int cols, F&& f) {
+  switch (row_mode<T>(cols)) {
+    case kRowEven: return f(std::integral_constant<int, kRowEven>{});
+    case kRowTail: return f(std::integral_constant<int, kRowTail>{});
+    default: return f(std::integral_constant<int, kRowTiny>{});
+  }
+}
+
+// Values [c, c + kVec) of a row of `cols`.  load() is one unconditional 16-byte load (tiny rows aside),
+// so that several are in flight at once: a branch with a conversion in it waits for each.  A tail's
+// vector is read so that it ends with the row, one past the row from the row's start; get() gives
+// its values as floats, shifted to their places, zeros past the row.
+template <typename T, int MODE>
+struct RowVec {
+  static constexpr int V = kVec<T>;
+  Pack<T> r;
+  __device__ __forceinline__ void load(const T* row, int c, int cols) {
+    if constexpr (MODE == kRowTiny) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) r.v[i] = c + i < cols ? row[c + i] : (T)0.0f;
+    } else {
+      r = load_pack(row + (c + V <= cols ? c : MODE == kRowTail ? cols - V : 0));
+    }
+  }
+  __device__ __forceinline__ void get(int c, int cols, float* out) const {
+    const int n = cols - c;
+    if constexpr (MODE == kRowTail) {
+      const int s = n > 0 && n < V ? V - n : 0;
+      uint32_t w[4];
+      memcpy(w, &r, 16);
+      constexpr int kTop = sizeof(T) == 2 ? 4 : 2;   // elements of two words
+      if (s & kTop) {
+        w[0] = w[2];
+        w[1] = w[3];
+      }
+      if (s & (kTop / 2)) {
+        w[0] = w[1];
+        w[1] = w[2];
+        w[2] = w[3];
+      }
+      if (sizeof(T) == 2 && (s & 1)) {
+        w[0] = w[0] >> 16 | w[1] << 16;
+        w[1] = w[1] >> 16 | w[2] << 16;
+        w[2] = w[2] >> 16 | w[3] << 16;
+        w[3] >>= 16;
+      }
+      Pack<T> q;
+      memcpy(&q, w, 16);
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] = i < n ? (float)q.v[i] : 0.0f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] = n > 0 ? (float)r.v[i] : 0.0f;
+    }
+  }
+};
+// The first n values at p as floats, zeros behind (joins of partial sums; n >= 1).
 template <typename T>
 __device__ __forceinline__ void load_row(const T* p, int n, float* out) {
+  Pack<T> r;
   if (n >= kVec<T>) {
-    const Pack<T> r = load_pack(p);
-#pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) out[i] = (float)r.v[i];
+    r = load_pack(p);
   } else {
 #pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) out[i] = i < n ? (float)p[i] : 0.0f;
+    for (int i = 0; i < kVec<T>; ++i) r.v[i] = i < n ? p[i] : (T)0.0f;
   }
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) out[i] = (float)r.v[i];
 }
 template <typename T>
 __device__ __forceinline__ void store_row(T* p, int n, const float* in) {

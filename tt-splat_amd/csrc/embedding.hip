@@ -8,12 +8,12 @@
 // Gradient: the tokens are sorted by id, stably, so each row's sum runs over its tokens in token
 // order whatever the launch does: no float atomics, the same inputs give the same bits.
 //   sort    least-significant-digit radix sort of (id, position), digits of up to 11 bits: one pass up
-//           to V = 2047, two up to 4M.  A pass is a histogram per tile of 4096 tokens, a scan of each
+//           to V = 2047, two up to 4M.  A pass is a histogram per tile of 1024 tokens, a scan of each
 //           digit's column of counts, and a scatter that ranks a tile's tokens (lanes with an equal
 //           digit find each other by ballots).  Up to 4096 tokens one block does it all in LDS.
 //   chunks  64 sorted tokens at a time: where one id fills a chunk, the chunk's sum.  The same again
 //           over 64 chunks where one id fills them all.
-//   rows    a row's sum: its tokens outside full chunks, the sums of its full chunks outside full
+//   rows    a row's sum, by one lane group or several: its tokens outside full chunks, the sums of its full chunks outside full
 //           spans of 64, the sums of those spans.  A row that a million tokens name is so read by
 //           the whole device in the chunk pass, and no row walks more than 128 tokens, 128 chunks
 //           and tokens / 4096 spans.
@@ -25,8 +25,10 @@ namespace tts {
 
 constexpr int kEmbBlock = 256;
 constexpr int kEmbWaves = kEmbBlock / 64;
-constexpr int kTileTokens = 4096;                      // tokens a block sorts
-constexpr int kTokPerThread = kTileTokens / kEmbBlock;
+constexpr int kSmallPer = 16, kSmallTokens = kSmallPer * kEmbBlock;   // one block sorts up to 4096 tokens
+// Tokens a thread and a block of a pass over more: 1024 a block fill the card from 260 000 tokens on
+// (4096 a block: scatter of 100 000 tokens 15.4 -> TODO us, of a million 28.0 -> TODO).
+constexpr int kPassPer = 4, kPassTokens = kPassPer * kEmbBlock;
 constexpr int kMaxDigitBits = 11;
 constexpr int kMaxBins = 1 << kMaxDigitBits;
 constexpr int kChunk = 64;                             // sorted tokens a chunk, chunks a span
@@ -39,7 +41,7 @@ __device__ __forceinline__ uint32_t token_key(const I* ids, int64_t t, uint32_t 
   return id >= 0 && id < (I)V ? (uint32_t)id : V;
 }
 
-template <typename T, typename I>
+template <typename T, typename I, int MODE>
 __global__ __launch_bounds__(kEmbBlock) void k_emb_fwd(const T* __restrict__ table, uint32_t V,
                                                        int D, const I* __restrict__ ids, int64_t N,
                                                        float scale, T* __restrict__ out, int L) {
@@ -53,7 +55,9 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_fwd(const T* __restrict__ tab
     for (int c = lig * VE; c < D; c += L * VE) {
       float v[VE] = {};
       if (k < V) {
-        load_row(src + c, D - c, v);
+        RowVec<T, MODE> r;
+        r.load(src, c, D);
+        r.get(c, D, v);
 #pragma unroll
         for (int i = 0; i < VE; ++i) v[i] *= scale;
       }
@@ -85,16 +89,21 @@ struct SortBuf {
 
 // Ranks a tile's keys for one digit: cnt[wave][bin] ends as the wave's count of each digit, rank[r]
 // is the token's place among the wave's tokens of its digit.  Token r of a lane is at
-// wave * 1024 + r * 64 + lane: order along the tile is (wave, r, lane).
-__device__ __forceinline__ void rank_tile(const uint32_t (&key)[kTokPerThread], int n, int shift,
-                                          int bits, int* cnt, int (&rank)[kTokPerThread]) {
+// wave * 64 PER + r * 64 + lane: order along the tile is (wave, r, lane).
+template <int PER>
+__device__ __forceinline__ int tile_token(int r) {
+  return (int)(threadIdx.x >> 6) * (64 * PER) + r * 64 + (int)(threadIdx.x & 63);
+}
+template <int PER>
+__device__ __forceinline__ void rank_tile(const uint32_t (&key)[PER], int n, int shift, int bits,
+                                          int* cnt, int (&rank)[PER]) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, bins = 1 << bits;
   for (int i = threadIdx.x; i < kEmbWaves * bins; i += kEmbBlock) cnt[i] = 0;
   __syncthreads();
   volatile int* c = cnt + wave * bins;
 #pragma unroll
-  for (int r = 0; r < kTokPerThread; ++r) {
-    const bool on = wave * (kTileTokens / kEmbWaves) + r * 64 + lane < n;
+  for (int r = 0; r < PER; ++r) {
+    const bool on = tile_token<PER>(r) < n;
     const uint32_t d = (key[r] >> shift) & (bins - 1);
     const uint64_t m = same_digit(d, bits, on);
     const int before = __popcll(m & ((1ull << lane) - 1));
@@ -115,8 +124,8 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_sort_small(const I* __restric
                                                               int32_t* __restrict__ opos,
                                                               int2* __restrict__ range) {
   __shared__ int cnt[kEmbWaves * kMaxBins];
-  __shared__ uint32_t skey[kTileTokens];
-  __shared__ uint16_t spos[kTileTokens];
+  __shared__ uint32_t skey[kSmallTokens];
+  __shared__ uint16_t spos[kSmallTokens];
   __shared__ int tmp[kEmbWaves];
   if (gridDim.x > 1) {
     if (blockIdx.x > 0) {
@@ -128,12 +137,12 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_sort_small(const I* __restric
   } else {
     for (uint32_t v = threadIdx.x; v < V; v += kEmbBlock) range[v] = make_int2(0, 0);
   }
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, bins = 1 << bits;
-  uint32_t key[kTokPerThread];
-  int pos[kTokPerThread], rank[kTokPerThread];
+  const int wave = threadIdx.x >> 6, bins = 1 << bits;
+  uint32_t key[kSmallPer];
+  int pos[kSmallPer], rank[kSmallPer];
 #pragma unroll
-  for (int r = 0; r < kTokPerThread; ++r) {
-    const int t = wave * (kTileTokens / kEmbWaves) + r * 64 + lane;
+  for (int r = 0; r < kSmallPer; ++r) {
+    const int t = tile_token<kSmallPer>(r);
     key[r] = t < N ? token_key(ids, t, V) : 0;
     pos[r] = t;
   }
@@ -157,8 +166,8 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_sort_small(const I* __restric
         }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kTokPerThread; ++r) {
-      const int t = wave * (kTileTokens / kEmbWaves) + r * 64 + lane;
+    for (int r = 0; r < kSmallPer; ++r) {
+      const int t = tile_token<kSmallPer>(r);
       if (t < N) {
         const int to = cnt[wave * bins + ((key[r] >> (p * bits)) & (bins - 1))] + rank[r];
         skey[to] = key[r];
@@ -167,8 +176,8 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_sort_small(const I* __restric
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kTokPerThread; ++r) {
-      const int t = wave * (kTileTokens / kEmbWaves) + r * 64 + lane;
+    for (int r = 0; r < kSmallPer; ++r) {
+      const int t = tile_token<kSmallPer>(r);
       if (t < N) {
         key[r] = skey[t];
         pos[r] = spos[t];
@@ -177,8 +186,8 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_sort_small(const I* __restric
     __syncthreads();
   }
 #pragma unroll
-  for (int r = 0; r < kTokPerThread; ++r) {
-    const int t = wave * (kTileTokens / kEmbWaves) + r * 64 + lane;
+  for (int r = 0; r < kSmallPer; ++r) {
+    const int t = tile_token<kSmallPer>(r);
     if (t < N) {
       okey[t] = key[r];
       opos[t] = pos[r];
@@ -208,15 +217,15 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_hist(const I* __restrict__ id
          v += (int64_t)gridDim.x * kEmbBlock)
       range[v] = make_int2(0, 0);
   __syncthreads();
-  const int64_t t0 = (int64_t)blockIdx.x * kTileTokens;
-  uint32_t k[kTokPerThread];
+  const int64_t t0 = (int64_t)blockIdx.x * kPassTokens;
+  uint32_t k[kPassPer];
 #pragma unroll
-  for (int r = 0; r < kTokPerThread; ++r) {
+  for (int r = 0; r < kPassPer; ++r) {
     const int64_t t = t0 + r * kEmbBlock + threadIdx.x;
     k[r] = t < N ? pass_key(ids, key, t, V) : 0;
   }
 #pragma unroll
-  for (int r = 0; r < kTokPerThread; ++r)
+  for (int r = 0; r < kPassPer; ++r)
     if (t0 + r * kEmbBlock + threadIdx.x < N) atomicAdd(&cnt[(k[r] >> shift) & (bins - 1)], 1);
   __syncthreads();
   for (int i = threadIdx.x; i < bins; i += kEmbBlock)
@@ -248,14 +257,14 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_scatter(
   __shared__ int cnt[kEmbWaves * kMaxBins];
   __shared__ int tmp[kEmbWaves];
   const int bins = 1 << bits;
-  const int64_t t0 = (int64_t)blockIdx.x * kTileTokens;
-  const int n = (int)(N - t0 < kTileTokens ? N - t0 : kTileTokens);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  uint32_t k[kTokPerThread];
-  int p[kTokPerThread], rank[kTokPerThread];
+  const int64_t t0 = (int64_t)blockIdx.x * kPassTokens;
+  const int n = (int)(N - t0 < kPassTokens ? N - t0 : kPassTokens);
+  const int wave = threadIdx.x >> 6;
+  uint32_t k[kPassPer];
+  int p[kPassPer], rank[kPassPer];
 #pragma unroll
-  for (int r = 0; r < kTokPerThread; ++r) {
-    const int i = wave * (kTileTokens / kEmbWaves) + r * 64 + lane;
+  for (int r = 0; r < kPassPer; ++r) {
+    const int i = tile_token<kPassPer>(r);
     k[r] = i < n ? pass_key(ids, key, t0 + i, V) : 0;
     p[r] = i < n ? (pos ? pos[t0 + i] : (int)(t0 + i)) : 0;
   }
@@ -280,8 +289,8 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_scatter(
     }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kTokPerThread; ++r) {
-    const int i = wave * (kTileTokens / kEmbWaves) + r * 64 + lane;
+  for (int r = 0; r < kPassPer; ++r) {
+    const int i = tile_token<kPassPer>(r);
     if (i < n) {
       const int to = cnt[wave * bins + ((k[r] >> shift) & (bins - 1))] + rank[r];
       okey[to] = k[r];
@@ -290,40 +299,43 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_scatter(
   }
 }
 
-// Sum of rows src[at(0..count)) over the columns [c, c + V) by one lane group, eight loads in flight.
-template <typename T, typename At>
-__device__ __forceinline__ void add_rows(const T* src, int D, int c, int64_t first, int64_t last,
-                                         int64_t step, At at, float* acc) {
-  constexpr int V = kVec<T>;
-  const int n = D - c;
-  int64_t i = first;
-  for (; i + 7 * step < last; i += 8 * step) {
-    float v[8][V];
+// acc += rows src[at(i)], i = first, first + step, .. < last, over the columns [c, c + V) by one lane
+// group: eight rows in flight.  Past the last row nothing is read.
+template <typename T, int MODE, typename At>
+__device__ __forceinline__ void add_rows(const T* src, int D, int c, int first, int last, int step,
+                                         At at, float* acc) {
+  constexpr int V = kVec<T>, B = 8;
+  for (int i = first; i < last; i += B * step) {
+    RowVec<T, MODE> r[B];
+    int p[B];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) load_row(src + (int64_t)at(i + u * step) * D + c, n, v[u]);
+    for (int u = 0; u < B; ++u)
+      if (i + u * step < last) p[u] = at(i + u * step);
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
+    for (int u = 0; u < B; ++u)
+      if (i + u * step < last) r[u].load(src + (int64_t)p[u] * D, c, D);
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += v[u][j];
-  }
-  for (; i < last; i += step) {
-    float v[V];
-    load_row(src + (int64_t)at(i) * D + c, n, v);
+    for (int u = 0; u < B; ++u) {
+      if (i + u * step < last) {
+        float v[V];
+        r[u].get(c, D, v);
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] += v[j];
+        for (int j = 0; j < V; ++j) acc[j] += v[j];
+      }
+    }
   }
 }
 
-// Sum over the wave's 64 / L groups, the same in each.
+// Sum over groups of L lanes up to `end` lanes, the same in each.
 template <int N>
-__device__ __forceinline__ void add_groups(float (&acc)[N], int L) {
-  for (int o = L; o < 64; o *= 2)
+__device__ __forceinline__ void add_groups(float (&acc)[N], int L, int end = 64) {
+  for (int o = L; o < end; o *= 2)
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] += __shfl_xor(acc[j], o, 64);
 }
 
 // Chunk c's sum where one row's tokens fill it (a wave a chunk), and the rows' ranges.
-template <typename T>
+template <typename T, int MODE>
 __global__ __launch_bounds__(kEmbBlock) void k_emb_chunk(const uint32_t* __restrict__ key,
                                                          const int32_t* __restrict__ pos, int64_t N,
                                                          uint32_t V, int D,
@@ -349,14 +361,15 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_chunk(const uint32_t* __restr
   for (int cb = 0; cb < D; cb += L * VE) {
     const int c = cb + lig * VE;
     float acc[VE] = {};
+#pragma unroll 8
     for (int i0 = 0; i0 < kChunk; i0 += G) {   // all lanes together: p comes from other lanes
       const int q = __shfl(p, i0 + grp, 64);
-      if (c < D) {
-        float v[VE];
-        load_row(dy + (int64_t)q * D + c, D - c, v);
+      RowVec<T, MODE> r;
+      r.load(dy + (int64_t)q * D, c, D);
+      float v[VE];
+      r.get(c, D, v);
 #pragma unroll
-        for (int j = 0; j < VE; ++j) acc[j] += v[j];
-      }
+      for (int j = 0; j < VE; ++j) acc[j] += v[j];
     }
     add_groups(acc, L);
     if (grp == 0 && c < D)
@@ -365,6 +378,7 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_chunk(const uint32_t* __restr
 }
 
 // Span s's sum where one row fills its 64 chunks (a wave a span).
+template <int MODE>
 __global__ __launch_bounds__(kEmbBlock) void k_emb_span(const uint32_t* __restrict__ key, int64_t N,
                                                         uint32_t V, int D,
                                                         const float* __restrict__ chunk,
@@ -379,56 +393,59 @@ __global__ __launch_bounds__(kEmbBlock) void k_emb_span(const uint32_t* __restri
     const int c = cb + lig * VE;
     float acc[VE] = {};
     if (c < D)
-      add_rows(chunk, D, c, s * kChunk + grp, (s + 1) * kChunk, G, [](int64_t i) { return i; }, acc);
+      add_rows<float, MODE>(chunk, D, c, (int)s * kChunk + grp, (int)(s + 1) * kChunk, G,
+                            [](int i) { return i; }, acc);
     add_groups(acc, L);
     if (grp == 0 && c < D)
       for (int j = 0; j < VE && c + j < D; ++j) span[s * D + c + j] = acc[j];
   }
 }
 
-// dW's rows: L lanes a row, in the fixed order head tokens, head chunks, spans, tail chunks, tail tokens.
-template <typename T>
+// dW's rows: G groups of L lanes a row, each in the fixed order head tokens, tail tokens, head chunks,
+// spans, tail chunks, of which it takes every G-th; the groups' sums are joined in a tree.
+// MODE, FMODE: row modes of the gradient's and of the partial sums' rows.
+template <typename T, int MODE, int FMODE>
 __global__ __launch_bounds__(kEmbBlock) void k_emb_rows(const int2* __restrict__ range,
                                                         const int32_t* __restrict__ pos,
                                                         uint32_t V, int D,
                                                         const T* __restrict__ dy,
                                                         const float* __restrict__ chunk,
                                                         const float* __restrict__ span, float scale,
-                                                        T* __restrict__ dw, int L) {
+                                                        T* __restrict__ dw, int L, int G) {
   constexpr int VE = kVec<T>, VF = kVec<float>;
-  const int lig = threadIdx.x & (L - 1), per = kEmbBlock / L;
-  for (int64_t v = (int64_t)blockIdx.x * per + threadIdx.x / L; v < V;
+  const int lig = threadIdx.x & (L - 1), g = threadIdx.x / L & (G - 1), per = kEmbBlock / (L * G);
+  for (int64_t v = (int64_t)blockIdx.x * per + threadIdx.x / (L * G); v < V;
        v += (int64_t)gridDim.x * per) {
     const int2 r = range[v];
-    const int64_t b = r.x, e = r.y;
-    const int64_t c0 = (b + kChunk - 1) / kChunk, c1 = e / kChunk;   // full chunks [c0, c1)
-    const int64_t s0 = (b + kSpan - 1) / kSpan, s1 = e / kSpan;      // full spans [s0, s1)
+    // first / last places of: head tokens, head chunks, spans, tail chunks, tail tokens
+    const int b = r.x, e = r.y;
+    const int c0 = (b + kChunk - 1) / kChunk, c1 = e / kChunk;   // full chunks [c0, c1)
+    const int s0 = (b + kSpan - 1) / kSpan, s1 = e / kSpan;      // full spans [s0, s1)
     const bool chunks = c0 < c1, spans = s0 < s1;
-    for (int c = lig * VE; c < D; c += L * VE) {
+    const int tb[2] = {b, chunks ? c1 * kChunk : e}, te[2] = {chunks ? c0 * kChunk : e, e};
+    const int cb2[2] = {c0, spans ? s1 * kChunk : c1}, ce[2] = {spans ? s0 * kChunk : c1, c1};
+    for (int cb = 0; cb < D; cb += L * VE) {
+      const int c = cb + lig * VE;
       float acc[VE] = {};
-      auto tokens = [&](int64_t i, int64_t j) {
-        add_rows(dy, D, c, i, j, 1, [&](int64_t t) { return pos[t]; }, acc);
-      };
-      auto floats = [&](const float* src, int64_t i, int64_t j) {
-        for (int h = 0; h < VE && c + h < D; h += VF)
-          add_rows(src, D, c + h, i, j, 1, [](int64_t t) { return t; }, acc + h);
-      };
-      if (!chunks) {
-        tokens(b, e);
-      } else {
-        tokens(b, c0 * kChunk);
-        if (!spans) {
-          floats(chunk, c0, c1);
-        } else {
-          floats(chunk, c0, s0 * kChunk);
-          floats(span, s0, s1);
-          floats(chunk, s1 * kChunk, c1);
+      if (c < D) {
+        for (int k = 0; k < 2; ++k)
+          add_rows<T, MODE>(dy, D, c, tb[k] + g, te[k], G, [&](int t) { return pos[t]; }, acc);
+        if (chunks) {
+          for (int k = 0; k < 3; ++k) {
+            const float* src = k == 1 ? span : chunk;
+            const int i = k == 1 ? s0 : cb2[k / 2], j = k == 1 ? s1 : ce[k / 2];
+            if (k == 1 && !spans) continue;
+#pragma unroll
+            for (int h = 0; h < VE; h += VF)
+              if (c + h < D)
+                add_rows<float, FMODE>(src, D, c + h, i + g, j, G, [](int t) { return t; }, acc + h);
+          }
         }
-        tokens(c1 * kChunk, e);
       }
+      add_groups(acc, L, L * G);
 #pragma unroll
       for (int j = 0; j < VE; ++j) acc[j] *= scale;
-      store_row(dw + v * D + c, D - c, acc);
+      if (g == 0 && c < D) store_row(dw + v * D + c, D - c, acc);
     }
   }
 }
@@ -444,14 +461,14 @@ inline void emb_digits(uint32_t V, int* passes, int* bits) {
 inline size_t emb_layout(int64_t N, int64_t V, int D, char* base, SortBuf* w) {
   int passes, bits;
   emb_digits((uint32_t)V, &passes, &bits);
-  const size_t n = (size_t)N, tiles = (n + kTileTokens - 1) / kTileTokens;
+  const size_t n = (size_t)N, tiles = (n + kPassTokens - 1) / kPassTokens;
   size_t off = 0;
   auto take = [&](size_t bytes) {
     char* p = base ? base + off : nullptr;
     off += align256(bytes);
     return p;
   };
-  const bool big = N > kTileTokens;
+  const bool big = N > kSmallTokens;
   char* k0 = take(4 * n);
   char* k1 = take(big && passes > 1 ? 4 * n : 0);
   char* p0 = take(4 * n);
@@ -493,12 +510,12 @@ int emb_bwd(const T* dy, const I* ids, int64_t N, int64_t V, int D, float scale,
   emb_digits((uint32_t)V, &passes, &bits);
   const uint32_t v32 = (uint32_t)V;
   int cur = 0;
-  if (N <= kTileTokens) {
+  if (N <= kSmallTokens) {
     const int nb = 1 + (int)(V > 4096 ? (V / 4096 < 256 ? V / 4096 : 256) : 0);
     k_emb_sort_small<I><<<nb, kEmbBlock, 0, stream>>>(ids, (int)N, v32, passes, bits, w.key[0],
                                                       w.pos[0], w.range);
   } else {
-    const int tiles = (int)((N + kTileTokens - 1) / kTileTokens);
+    const int tiles = (int)((N + kPassTokens - 1) / kPassTokens);
     cur = 1;
     for (int p = 0; p < passes; ++p) {
       const uint32_t* key = p ? w.key[cur] : nullptr;
@@ -514,17 +531,33 @@ int emb_bwd(const T* dy, const I* ids, int64_t N, int64_t V, int D, float scale,
   const int L = row_lanes((D - 1) / kVec<T> + 1), Lf = row_lanes((D - 1) / kVec<float> + 1);
   if (N > 0) {
     const int64_t nch = (N + kChunk - 1) / kChunk;
-    k_emb_chunk<T><<<(int)((nch + kEmbWaves - 1) / kEmbWaves), kEmbBlock, 0, stream>>>(
-        w.key[cur], w.pos[cur], N, v32, D, dy, w.chunk, w.range, L);
+    by_row_mode<T>(D, [&](auto mode) {
+      k_emb_chunk<T, mode()><<<(int)((nch + kEmbWaves - 1) / kEmbWaves), kEmbBlock, 0, stream>>>(
+          w.key[cur], w.pos[cur], N, v32, D, dy, w.chunk, w.range, L);
+      return 0;
+    });
     const int64_t nsp = N / kSpan;
     if (nsp > 0)
-      k_emb_span<<<(int)((nsp + kEmbWaves - 1) / kEmbWaves), kEmbBlock, 0, stream>>>(
-          w.key[cur], N, v32, D, w.chunk, w.span, Lf);
+      by_row_mode<float>(D, [&](auto mode) {
+        k_emb_span<mode()><<<(int)((nsp + kEmbWaves - 1) / kEmbWaves), kEmbBlock, 0, stream>>>(
+            w.key[cur], N, v32, D, w.chunk, w.span, Lf);
+        return 0;
+      });
   }
-  const int per = kEmbBlock / L;
-  k_emb_rows<T><<<emb_blocks((V + per - 1) / per), kEmbBlock, 0, stream>>>(
-      w.range, w.pos[cur], v32, D, dy, w.chunk, w.span, scale, dw, L);
-  return launch_status();
+  // groups a row: one for every two tokens of a mean row, as far as a wave holds them
+  int G = 1;
+  while (2 * G * L <= 64 && (int64_t)4 * G * V <= N) G *= 2;
+  const int per = kEmbBlock / (L * G);
+  return by_row_mode<T>(D, [&](auto mode) {
+    return by_row_mode<float>(D, [&](auto fmode) {
+      // an even row of a half type is even in fp32, a tiny one in fp32 is tiny in the half types
+      if constexpr ((mode() != kRowEven || fmode() == kRowEven) &&
+                    (fmode() != kRowTiny || mode() == kRowTiny))
+        k_emb_rows<T, mode(), fmode()><<<emb_blocks((V + per - 1) / per), kEmbBlock, 0, stream>>>(
+            w.range, w.pos[cur], v32, D, dy, w.chunk, w.span, scale, dw, L, G);
+      return launch_status();
+    });
+  });
 }
 
 }  // namespace tts
@@ -545,13 +578,15 @@ int tts_embedding_fwd(const void* table, int64_t V, int D, const void* ids, int 
     const int nb = emb_blocks((N + per - 1) / per);
     const T* tb = static_cast<const T*>(table);
     T* o = static_cast<T*>(out);
-    if (ids64)
-      k_emb_fwd<T, int64_t><<<nb, kEmbBlock, 0, stream>>>(
-          tb, (uint32_t)V, D, static_cast<const int64_t*>(ids), N, scale, o, L);
-    else
-      k_emb_fwd<T, int32_t><<<nb, kEmbBlock, 0, stream>>>(
-          tb, (uint32_t)V, D, static_cast<const int32_t*>(ids), N, scale, o, L);
-    return launch_status();
+    return by_row_mode<T>(D, [&](auto mode) {
+      if (ids64)
+        k_emb_fwd<T, int64_t, mode()><<<nb, kEmbBlock, 0, stream>>>(
+            tb, (uint32_t)V, D, static_cast<const int64_t*>(ids), N, scale, o, L);
+      else
+        k_emb_fwd<T, int32_t, mode()><<<nb, kEmbBlock, 0, stream>>>(
+            tb, (uint32_t)V, D, static_cast<const int32_t*>(ids), N, scale, o, L);
+      return launch_status();
+    });
   });
 }
 

@@ -23,28 +23,39 @@ constexpr int kLnBlock = 256;
 constexpr int kLnWaves = kLnBlock / 64;
 constexpr int kLnFwdBlocks = 2048;  // eight blocks a CU walk the rows
 constexpr int kLnBwdBlocks = 1024;  // four a CU; each leaves one row of partials behind
+constexpr int kLnShare = 4;         // rows a lane group or more where the card is full without
 constexpr int kLnRegVecs = 256;     // rows of up to this many vectors stay in registers
 
-// Weights of one lane's vectors, `fill` where there is none.
-template <typename T, int L, int NV>
+// Weights of one lane's vectors at [c, c + kVec), `fill` where there is none.
+template <typename T, int MODE>
+__device__ __forceinline__ void ln_weight(const void* w, int wf32, int c, int cols, float fill,
+                                          float* out) {
+  constexpr int V = kVec<T>, VF = kVec<float>;
+  if (!w) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = fill;
+  } else if (wf32) {
+#pragma unroll
+    for (int h = 0; h < V; h += VF) {   // a tiny row of a half type may hold more than four values
+      RowVec<float, MODE> r;
+      r.load(static_cast<const float*>(w), c + h, cols);
+      r.get(c + h, cols, out + h);
+    }
+  } else {
+    RowVec<T, MODE> r;
+    r.load(static_cast<const T*>(w), c, cols);
+    r.get(c, cols, out);
+  }
+}
+template <typename T, int L, int NV, int MODE>
 __device__ __forceinline__ void ln_load_weight(const void* w, int wf32, int cols, int lig,
                                                float fill, float (&out)[NV][kVec<T>]) {
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) {
-      const int c = (lig + j * L) * kVec<T> + i;
-      out[j][i] = fill;
-      if (w && c < cols) {
-        if (wf32)
-          out[j][i] = static_cast<const float*>(w)[c];
-        else
-          out[j][i] = (float)static_cast<const T*>(w)[c];
-      }
-    }
+    ln_weight<T, MODE>(w, wf32, (lig + j * L) * kVec<T>, cols, fill, out[j]);
 }
 
-template <typename T, int L, int NV>
+template <typename T, int L, int NV, int MODE>
 __global__ __launch_bounds__(kLnBlock) void k_ln_fwd(const T* __restrict__ x, int64_t xs,
                                                      const void* __restrict__ w,
                                                      const void* __restrict__ b, int wf32,
@@ -53,14 +64,17 @@ __global__ __launch_bounds__(kLnBlock) void k_ln_fwd(const T* __restrict__ x, in
   constexpr int V = kVec<T>, G = kLnBlock / L;
   const int lig = threadIdx.x & (L - 1), grp = threadIdx.x / L;
   float wt[NV][V], bi[NV][V];
-  ln_load_weight<T, L, NV>(w, wf32, cols, lig, 1.0f, wt);
-  ln_load_weight<T, L, NV>(b, wf32, cols, lig, 0.0f, bi);
+  ln_load_weight<T, L, NV, MODE>(w, wf32, cols, lig, 1.0f, wt);
+  ln_load_weight<T, L, NV, MODE>(b, wf32, cols, lig, 0.0f, bi);
   const float inv = 1.0f / (float)cols;
   for (int64_t row = (int64_t)blockIdx.x * G + grp; row < rows; row += (int64_t)gridDim.x * G) {
     const T* xr = x + row * xs;
     float v[NV][V], s = 0.0f;
+    RowVec<T, MODE> rv[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) load_row(xr + (lig + j * L) * V, cols - (lig + j * L) * V, v[j]);
+    for (int j = 0; j < NV; ++j) rv[j].load(xr, (lig + j * L) * V, cols);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) rv[j].get((lig + j * L) * V, cols, v[j]);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -119,15 +133,13 @@ __global__ __launch_bounds__(kLnBlock) void k_ln_fwd_wide(const T* __restrict__ 
     }
     const float r = 1.0f / sqrtf(block_sum256(q, tmp) * inv + eps);
     for (int64_t c = (int64_t)threadIdx.x * V; c < cols; c += kLnBlock * V) {
-      float wt[1][V], bi[1][V];
+      float wt[V], bi[V];
       const int n = (int)(cols - c);
       load_row(xr + c, n, v);
-      ln_load_weight<T, 1, 1>(w ? static_cast<const char*>(w) + c * (wf32 ? 4 : sizeof(T)) : w,
-                              wf32, n, 0, 1.0f, wt);
-      ln_load_weight<T, 1, 1>(b ? static_cast<const char*>(b) + c * (wf32 ? 4 : sizeof(T)) : b,
-                              wf32, n, 0, 0.0f, bi);
+      ln_weight<T, kRowTail>(w, wf32, (int)c, cols, 1.0f, wt);
+      ln_weight<T, kRowTail>(b, wf32, (int)c, cols, 0.0f, bi);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = (v[i] - m) * r * wt[0][i] + bi[0][i];
+      for (int i = 0; i < V; ++i) v[i] = (v[i] - m) * r * wt[i] + bi[i];
       store_row(yr + c, n, v);
     }
     if (stats && threadIdx.x == 0) stats[row] = make_float2(m, r);
@@ -135,7 +147,7 @@ __global__ __launch_bounds__(kLnBlock) void k_ln_fwd_wide(const T* __restrict__ 
 }
 
 // dx of the block's rows and its partial sums of dy xh and dy, part[block][2][cols].
-template <typename T, int L, int NV>
+template <typename T, int L, int NV, int MODE>
 __global__ __launch_bounds__(kLnBlock) void k_ln_bwd(const T* __restrict__ x, int64_t xs,
                                                      const void* __restrict__ w, int wf32,
                                                      const T* __restrict__ dy, int64_t dys,
@@ -146,18 +158,23 @@ __global__ __launch_bounds__(kLnBlock) void k_ln_bwd(const T* __restrict__ x, in
   __shared__ float red[2 * L * NV * V];
   const int lig = threadIdx.x & (L - 1), grp = threadIdx.x / L;
   float wt[NV][V], aw[NV][V] = {}, ab[NV][V] = {};
-  ln_load_weight<T, L, NV>(w, wf32, cols, lig, 1.0f, wt);
+  ln_load_weight<T, L, NV, MODE>(w, wf32, cols, lig, 1.0f, wt);
   const float inv = 1.0f / (float)cols;
   for (int64_t row = (int64_t)blockIdx.x * G + grp; row < rows; row += (int64_t)gridDim.x * G) {
     const T* xr = x + row * xs;
     const T* gr = dy + row * dys;
     const float2 st = stats[row];
     float v[NV][V], g[NV][V];
+    RowVec<T, MODE> rv[NV], rg[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (lig + j * L) * V;
-      load_row(xr + c, cols - c, v[j]);
-      load_row(gr + c, cols - c, g[j]);
+      rv[j].load(xr, (lig + j * L) * V, cols);
+      rg[j].load(gr, (lig + j * L) * V, cols);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      rv[j].get((lig + j * L) * V, cols, v[j]);
+      rg[j].get((lig + j * L) * V, cols, g[j]);
     }
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
@@ -232,18 +249,17 @@ __global__ __launch_bounds__(kLnBlock) void k_ln_bwd_wide(const T* __restrict__ 
     const T* gr = dy + row * dys;
     T* dr = dx + row * cols;
     const float2 st = stats[row];
-    float v[V], g[V], wt[1][V], s1 = 0.0f, s2 = 0.0f;
+    float v[V], g[V], wt[V], s1 = 0.0f, s2 = 0.0f;
     for (int pass = 0; pass < 2; ++pass) {
       for (int64_t c = (int64_t)threadIdx.x * V; c < cols; c += kLnBlock * V) {
         const int n = (int)(cols - c);
         load_row(xr + c, n, v);
         load_row(gr + c, n, g);
-        ln_load_weight<T, 1, 1>(w ? static_cast<const char*>(w) + c * (wf32 ? 4 : sizeof(T)) : w,
-                                wf32, n, 0, 1.0f, wt);
+        ln_weight<T, kRowTail>(w, wf32, (int)c, cols, 1.0f, wt);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           v[i] = (v[i] - st.x) * st.y;
-          g[i] *= wt[0][i];
+          g[i] *= wt[i];
           if (pass == 0) {
             s1 += g[i];
             s2 += g[i] * v[i];
@@ -318,34 +334,47 @@ __global__ __launch_bounds__(kLnBlock) void k_ln_join(const float* __restrict__ 
     static_cast<T*>(out)[i] = (T)s;
 }
 
+// Blocks of `per` rows at a time: as many as there are rows for up to two a CU, from there on each takes
+// kLnShare rows a lane group before another is added, so that weights are read (and partial sums
+// left) once for several rows.
+inline int64_t ln_blocks(int64_t rows, int64_t per, int64_t most) {
+  const int64_t want = (rows + per - 1) / per;
+  int64_t n = (want + kLnShare - 1) / kLnShare;
+  n = n < 512 ? 512 : n;
+  n = n < want ? n : want;
+  return n < most ? n : most;
+}
+
 // Blocks of the backward over `rows` rows of `cols` values of `esize` bytes.
 inline int ln_bwd_blocks(int64_t rows, int cols, int esize) {
   const int nvec = (int)(((int64_t)cols * esize + 15) / 16);
   if (rows <= 0) return 0;
-  const int64_t per = nvec > kLnRegVecs ? 1 : kLnBlock / row_lanes(nvec);
-  const int64_t want = (rows + per - 1) / per;
-  if (nvec <= kLnRegVecs) return (int)(want < kLnBwdBlocks ? want : kLnBwdBlocks);
+  if (nvec <= kLnRegVecs) return (int)ln_blocks(rows, kLnBlock / row_lanes(nvec), kLnBwdBlocks);
   // wide rows: strips of 256 vectors' columns by shares of at least 16 rows
   const int64_t strips = (nvec + kLnBlock - 1) / kLnBlock, share = (rows + 15) / 16;
   const int64_t cap = strips < kLnBwdBlocks ? kLnBwdBlocks / strips : 1;
   return (int)(share < cap ? share : cap);
 }
 
-// f(integral_constant L, integral_constant NV) for rows of nvec vectors.
-template <typename F>
-inline int ln_by_width(int nvec, F&& f) {
+// f(lanes a row, vectors a lane, row mode) for rows of nvec vectors.
+template <typename T, typename F>
+inline int ln_by_width(int cols, int nvec, F&& f) {
   using std::integral_constant;
-#define TTS_LN(L, NV) return f(integral_constant<int, L>{}, integral_constant<int, NV>{})
-  if (nvec <= 1) TTS_LN(1, 1);
-  if (nvec <= 2) TTS_LN(2, 1);
-  if (nvec <= 4) TTS_LN(4, 1);
-  if (nvec <= 8) TTS_LN(8, 1);
-  if (nvec <= 16) TTS_LN(16, 1);
-  if (nvec <= 32) TTS_LN(32, 1);
-  if (nvec <= 64) TTS_LN(64, 1);
-  if (nvec <= 128) TTS_LN(64, 2);
-  TTS_LN(64, 4);
+  return by_row_mode<T>(cols, [&](auto mode) {
+#define TTS_LN(L, NV) return f(integral_constant<int, L>{}, integral_constant<int, NV>{}, mode)
+    if constexpr (mode() != kRowTiny) {
+      if (nvec > 128) TTS_LN(64, 4);
+      if (nvec > 64) TTS_LN(64, 2);
+      if (nvec > 32) TTS_LN(64, 1);
+      if (nvec > 16) TTS_LN(32, 1);
+      if (nvec > 8) TTS_LN(16, 1);
+      if (nvec > 4) TTS_LN(8, 1);
+      if (nvec > 2) TTS_LN(4, 1);
+      if (nvec > 1) TTS_LN(2, 1);
+    }
+    TTS_LN(1, 1);
 #undef TTS_LN
+  });
 }
 
 }  // namespace tts
@@ -372,10 +401,9 @@ int tts_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, cons
                                                          cols, eps, yp, st);
       return launch_status();
     }
-    return ln_by_width(nvec, [&](auto L, auto NV) {
-      const int64_t per = kLnBlock / L(), want = (rows + per - 1) / per;
-      const int64_t nb = want < kLnFwdBlocks ? want : kLnFwdBlocks;
-      k_ln_fwd<T, L(), NV()><<<(int)nb, kLnBlock, 0, stream>>>(xp, x_stride, weight, bias, wf32,
+    return ln_by_width<T>(cols, nvec, [&](auto L, auto NV, auto mode) {
+      const int64_t nb = ln_blocks(rows, kLnBlock / L(), kLnFwdBlocks);
+      k_ln_fwd<T, L(), NV(), mode()><<<(int)nb, kLnBlock, 0, stream>>>(xp, x_stride, weight, bias, wf32,
                                                                rows, cols, eps, yp, st);
       return launch_status();
     });
@@ -417,8 +445,8 @@ int tts_layer_norm_bwd(const void* x, int64_t x_stride, const void* weight, cons
                                                      part);
       }
     } else if (rows > 0) {
-      ln_by_width(nvec, [&](auto L, auto NV) {
-        k_ln_bwd<T, L(), NV()><<<nb, kLnBlock, 0, stream>>>(xp, x_stride, weight, wf32, gp,
+      ln_by_width<T>(cols, nvec, [&](auto L, auto NV, auto mode) {
+        k_ln_bwd<T, L(), NV(), mode()><<<nb, kLnBlock, 0, stream>>>(xp, x_stride, weight, wf32, gp,
                                                             dy_stride, st, rows, cols, dxp, part);
         return 0;
       });

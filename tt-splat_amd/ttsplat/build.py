@@ -8,7 +8,7 @@ Flags
   -Xclang -target-feature -Xclang -packed-fp32-ops
                                    no packed-FP32 (v_pk_*_f32) codegen
   -ffp-contract=off (binning.hip)  binning keys are products and sums rounded one by one
-  -mllvm -amdgpu-mfma-vgpr-form (splat.hip)
+  -mllvm -amdgpu-mfma-vgpr-form (splat.hip, attention_*.hip)
                                    matrix-core results in VGPRs, not accumulator registers
 """
 import concurrent.futures as cf
@@ -30,7 +30,8 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",
           "-Wno-unused-command-line-argument", "-I", INCLUDE, "-I", CSRC]
 PER_FILE = {"binning.hip": ["-ffp-contract=off"],
             # matrix-core results straight into VGPRs (no accumulator-register copies)
-            "splat.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+            **{f: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+               for f in ("splat.hip", "attention_fwd.hip", "attention_dq.hip", "attention_dkv.hip")}}
 
 
 def hipcc():

@@ -1168,7 +1168,7 @@ def _attn_tensor(t, name, shape=None, dtype=None, device=None):
     st = t.stride()
     if st[3] != 1 and t.shape[3] > 1:
         raise ValueError(f"{name} must have a contiguous last axis")
-    return code, st[:3]
+    return code, st[:3] if t.shape[2] > 1 else (st[0], st[1], 0)
 
 
 def _attn_args(q, k, v, key_mask, causal, scale, out, dout=None, grads=(None, None, None)):
