@@ -292,7 +292,7 @@ def test_refusals():
                 lambda: kernels.attention_fwd(q, k, v, lse=torch.zeros(1, 4, 6, device="cuda"))):
         with pytest.raises(ValueError):
             bad()
-    shape, _ = kernels._attn_args(q, k, v, None, False, None, q, q, (q, k, v))
+    shape = kernels._attn_shape(q, k, v, q, None, False, 0.25, q, q, k, v)
     with pytest.raises(_lib.TTSError):       # no workspace
         _lib.call("tts_attention_bwd", shape, *(_lib.ptr(t) for t in (q, k, v)), None,
                   _lib.ptr(q), _lib.ptr(q), _lib.ptr(q), _lib.ptr(q), None, None, None, 0,

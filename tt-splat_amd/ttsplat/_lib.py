@@ -177,6 +177,18 @@ def call(name, *args):
     return code
 
 
+def entry(name):
+    """Entry point `name` as a callable that raises as call() does, its lookup done once.  Pointers
+    may be plain integers (Tensor.data_ptr())."""
+    fn = getattr(load(), name)
+
+    def run(*args):
+        code = fn(*args)
+        if code != 0:
+            raise TTSError(f"{name} failed with code {code}: {load().tts_strerror(code).decode()}")
+    return run
+
+
 def ptr(t):
     """Device pointer of a tensor (None -> NULL)."""
     return None if t is None else ctypes.c_void_p(t.data_ptr())
@@ -189,6 +201,11 @@ def stream():
     if not torch.cuda.is_initialized():
         return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+
+
+def raw_stream():
+    """The current stream as an integer, for callers that hold a GPU tensor (CUDA is initialised)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def require(t, name, dtype, shape=None, device=None):

@@ -6,7 +6,6 @@ keeps each row's log-sum-exp and no scores; the backward recomputes the probabil
 fp32, fp16 and bf16; the softmax and all sums are fp32.  Results are the same bits every time.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels
 
@@ -19,21 +18,23 @@ def _last_contiguous(t):
 
 
 class _Attention(torch.autograd.Function):
+    """mask: uint8 or None, checked with the rest by attention()."""
+
     @staticmethod
-    def forward(ctx, q, k, v, key_mask, causal, scale):
+    def forward(ctx, q, k, v, mask, causal, scale):
         lse = torch.empty(q.shape[:3], device=q.device, dtype=F32)
-        out = kernels.attention_fwd(q, k, v, key_mask, causal, scale, lse=lse)
-        ctx.save_for_backward(q, k, v, key_mask, out, lse)
+        out = kernels._attention_fwd(q, k, v, mask, causal, scale, kernels._attn_like(q), lse)
+        ctx.save_for_backward(q, k, v, mask, out, lse)
         ctx.meta = (causal, scale)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        q, k, v, key_mask, out, lse = ctx.saved_tensors
-        nq, nk, nv = ctx.needs_input_grad[:3]
-        grads = kernels.attention_bwd(q, k, v, out, lse, _last_contiguous(dout), key_mask, *ctx.meta,
-                                      nq, nk, nv)
+        q, k, v, mask, out, lse = ctx.saved_tensors
+        causal, scale = ctx.meta
+        nq, nk, nv, _, _, _ = ctx.needs_input_grad
+        grads = kernels._attention_bwd(q, k, v, mask, causal, scale, out, lse,
+                                       _last_contiguous(dout), nq, nk, nv)
         return (*grads, None, None, None)
 
 
@@ -45,5 +46,6 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None):
     i + Nk - Nq.  A row that sees no key gives zeros and no gradient."""
     q, k, v = _last_contiguous(q), _last_contiguous(k), _last_contiguous(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _Attention.apply(q, k, v, key_mask, bool(causal), scale)
+        mask, scale = kernels._attn_check(q, k, v, key_mask, scale, None)
+        return _Attention.apply(q, k, v, mask, bool(causal), scale)
     return kernels.attention_fwd(q, k, v, key_mask, causal, scale)

@@ -1024,7 +1024,26 @@ def wsr_dense_bwd(theta, o, color, keep, phi, bg, C, den, gC, workspace=None):
 
 
 # ------------------------------------------------------------- token networks beside a scene --
+# Calls of these are short beside Python's own time, so each entry point is looked up once, pointers
+# go as integers, and the autograd functions, whose forward has checked the arguments, call the
+# unchecked halves (_layer_norm_bwd and so on).
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ENTRIES = {}
+
+
+def _entry(name):
+    f = _ENTRIES.get(name)
+    if f is None:
+        f = _ENTRIES[name] = _lib.entry(name)
+    return f
+
+
+def _size(name, *args):
+    return getattr(_lib.load(), name)(*args)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _elem(t, name, device=None, dtype=None):
@@ -1077,40 +1096,46 @@ def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, y=None, stats=None):
     code = _norm_rows(x, "x")
     wcode = _norm_weights(x, weight, bias)
     R, D = x.shape
-    y = torch.empty(R, D, device=x.device, dtype=x.dtype) if y is None else y
-    require(y, "y", x.dtype, (R, D), x.device)
+    if y is None:
+        y = torch.empty(R, D, device=x.device, dtype=x.dtype)
+    else:
+        require(y, "y", x.dtype, (R, D), x.device)
     if stats is not None:
         require(stats, "stats", F32, (R, 2), x.device)
-    call("tts_layer_norm_fwd", ptr(x), x.stride(0), ptr(weight), ptr(bias), R, D, float(eps), code,
-         wcode, ptr(y), ptr(stats), stream())
+    _entry("tts_layer_norm_fwd")(x.data_ptr(), x.stride(0), _at(weight), _at(bias), R, D, eps, code,
+                                 wcode, y.data_ptr(), _at(stats), _lib.raw_stream())
     return y
+
+
+def _layer_norm_bwd(x, weight, dy, stats, dx, dweight, dbias, wt):
+    R, D = x.shape
+    dev, dt = x.device, x.dtype
+    gx = torch.empty(R, D, device=dev, dtype=dt) if dx else None
+    gw = torch.empty(D, device=dev, dtype=wt) if dweight else None
+    gb = torch.empty(D, device=dev, dtype=wt) if dbias else None
+    if not (dx or dweight or dbias):
+        return gx, gw, gb
+    code, ws, n = DTYPE_CODES[dt], None, 0
+    if dweight or dbias:
+        n = _size("tts_layer_norm_workspace_bytes", R, D, code)
+        ws = torch.empty(n, device=dev, dtype=U8)
+    _entry("tts_layer_norm_bwd")(x.data_ptr(), x.stride(0), _at(weight), dy.data_ptr(),
+                                 dy.stride(0), stats.data_ptr(), R, D, code, DTYPE_CODES[wt],
+                                 _at(gx), _at(gw), _at(gb), _at(ws), n, _lib.raw_stream())
+    return gx, gw, gb
 
 
 def layer_norm_bwd(x, weight, dy, stats, dx=True, dweight=True, dbias=True, w_dtype=None):
     """(dx, dweight, dbias) from the forward's stats; a False argument leaves that result out
     (None).  dweight and dbias are of weight's type (w_dtype where there is no weight)."""
-    code = _norm_rows(x, "x")
-    R, D = x.shape
-    dev = x.device
-    _norm_rows(dy, "dy", dev, x.dtype, x.shape)
-    wcode = _norm_weights(x, weight, None)
+    _norm_rows(x, "x")
+    _norm_rows(dy, "dy", x.device, x.dtype, x.shape)
+    _norm_weights(x, weight, None)
     wt = weight.dtype if weight is not None else (w_dtype or x.dtype)
     if wt != x.dtype and wt != F32:
         raise ValueError(f"w_dtype must be {x.dtype} or float32, got {wt}")
-    wcode = DTYPE_CODES[wt]
-    require(stats, "stats", F32, (R, 2), dev)
-    gx = torch.empty(R, D, device=dev, dtype=x.dtype) if dx else None
-    gw = torch.empty(D, device=dev, dtype=wt) if dweight else None
-    gb = torch.empty(D, device=dev, dtype=wt) if dbias else None
-    if not (dx or dweight or dbias):
-        return gx, gw, gb
-    ws, n = None, 0
-    if dweight or dbias:
-        n = _lib.load().tts_layer_norm_workspace_bytes(R, D, code)
-        ws = torch.empty(n, device=dev, dtype=U8)
-    call("tts_layer_norm_bwd", ptr(x), x.stride(0), ptr(weight), ptr(dy), dy.stride(0), ptr(stats),
-         R, D, code, wcode, ptr(gx), ptr(gw), ptr(gb), ptr(ws), n, stream())
-    return gx, gw, gb
+    require(stats, "stats", F32, (x.shape[0], 2), x.device)
+    return _layer_norm_bwd(x, weight, dy, stats, dx, dweight, dbias, wt)
 
 
 def _ids(ids, device):
@@ -1125,62 +1150,77 @@ def embedding_fwd(table, ids, scale=1.0, out=None):
     code = _elem(table, "table")
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError(f"table must be [V, D], got {tuple(table.shape)}")
-    require(table, "table", table.dtype)
+    if not table.is_contiguous():
+        raise ValueError("table must be contiguous")
     V, D = table.shape
     wide = _ids(ids, table.device)
     shape = (*ids.shape, D)
-    out = torch.empty(shape, device=table.device, dtype=table.dtype) if out is None else out
-    require(out, "out", table.dtype, shape, table.device)
-    call("tts_embedding_fwd", ptr(table), V, D, ptr(ids), wide, ids.numel(), float(scale), code,
-         ptr(out), stream())
+    if out is None:
+        out = torch.empty(shape, device=table.device, dtype=table.dtype)
+    else:
+        require(out, "out", table.dtype, shape, table.device)
+    _entry("tts_embedding_fwd")(table.data_ptr(), V, D, ids.data_ptr(), wide, ids.numel(), scale,
+                                code, out.data_ptr(), _lib.raw_stream())
+    return out
+
+
+def _embedding_bwd(dout, ids, V, scale, out=None, workspace=None):
+    D, N = dout.shape[-1], ids.numel()
+    if out is None:
+        out = torch.empty(V, D, device=dout.device, dtype=dout.dtype)
+    if workspace is None:
+        n = _size("tts_embedding_workspace_bytes", N, V, D)
+        workspace = torch.empty(n, device=dout.device, dtype=U8)
+    _entry("tts_embedding_bwd")(dout.data_ptr(), ids.data_ptr(), 1 if ids.dtype != I32 else 0, N, V,
+                                D, scale, DTYPE_CODES[dout.dtype], out.data_ptr(),
+                                workspace.data_ptr(), workspace.numel(), _lib.raw_stream())
     return out
 
 
 def embedding_bwd(dout, ids, V, scale=1.0, out=None, workspace=None):
     """dtable [V, D] = scale * the sum of dout's rows by id (fixed order, every row written)."""
-    code = _elem(dout, "dout")
-    wide = _ids(ids, dout.device)
+    _elem(dout, "dout")
+    _ids(ids, dout.device)
     if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape) or dout.shape[-1] < 1:
         raise ValueError(f"dout must be [*ids.shape, D], got {tuple(dout.shape)}")
     require(dout, "dout", dout.dtype)
-    D, N = dout.shape[-1], ids.numel()
-    out = torch.empty(V, D, device=dout.device, dtype=dout.dtype) if out is None else out
-    require(out, "out", dout.dtype, (V, D), dout.device)
-    if workspace is None:
-        n = _lib.load().tts_embedding_workspace_bytes(N, V, D)
-        workspace = torch.empty(n, device=dout.device, dtype=U8)
-    require(workspace, "workspace", U8, None, dout.device)
-    call("tts_embedding_bwd", ptr(dout), ptr(ids), wide, N, V, D, float(scale), code, ptr(out),
-         ptr(workspace), workspace.numel(), stream())
-    return out
+    if out is not None:
+        require(out, "out", dout.dtype, (V, dout.shape[-1]), dout.device)
+    if workspace is not None:
+        require(workspace, "workspace", U8, None, dout.device)
+    return _embedding_bwd(dout, ids, V, scale, out, workspace)
 
 
 _ATTN_SHAPE = struct.Struct("=33qd")   # tts_attention_shape
 _NO_STRIDE = (0, 0, 0)
 
 
+def _attn_stride(t):
+    st = t.stride()
+    return st[:3] if t.shape[2] > 1 else (st[0], st[1], 0)   # a single row's stride says nothing
+
+
 def _attn_tensor(t, name, shape=None, dtype=None, device=None):
-    code = _elem(t, name, device, dtype)
+    _elem(t, name, device, dtype)
     if t.dim() != 4:
         raise ValueError(f"{name} must be [batch, heads, length, head_dim], got {tuple(t.shape)}")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    st = t.stride()
-    if st[3] != 1 and t.shape[3] > 1:
+    if t.shape[3] > 1 and t.stride(3) != 1:
         raise ValueError(f"{name} must have a contiguous last axis")
-    return code, st[:3] if t.shape[2] > 1 else (st[0], st[1], 0)
+    return t
 
 
-def _attn_args(q, k, v, key_mask, causal, scale, out, dout=None, grads=(None, None, None)):
-    """The call's shape block, checked, and the mask as uint8."""
-    code, sq = _attn_tensor(q, "q")
+def _attn_check(q, k, v, key_mask, scale, out):
+    """Checked (mask as uint8 with a contiguous last axis, scale)."""
+    _attn_tensor(q, "q")
     dev, dt = q.device, q.dtype
-    _, sk = _attn_tensor(k, "k", None, dt, dev)
+    _attn_tensor(k, "k", None, dt, dev)
     B, Hq, Nq, D = q.shape
     _, Hkv, Nk, _ = k.shape
     if k.shape[0] != B or k.shape[3] != D:
         raise ValueError(f"k has shape {tuple(k.shape)}, expected [{B}, heads, keys, {D}]")
-    _, sv = _attn_tensor(v, "v", k.shape, dt, dev)
+    _attn_tensor(v, "v", k.shape, dt, dev)
     if Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads are not a multiple of {Hkv} key heads")
     if not 1 <= D <= 128:
@@ -1188,8 +1228,8 @@ def _attn_args(q, k, v, key_mask, causal, scale, out, dout=None, grads=(None, No
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    _, so = _attn_tensor(out, "out", q.shape, dt, dev)
-    ms = 0
+    if out is not None:
+        _attn_tensor(out, "out", q.shape, dt, dev)
     if key_mask is not None:
         if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in (torch.bool, U8):
             raise ValueError("key_mask must be a bool or uint8 tensor")
@@ -1200,12 +1240,17 @@ def _attn_args(q, k, v, key_mask, causal, scale, out, dout=None, grads=(None, No
             key_mask = key_mask.view(U8)
         if Nk > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
-        ms = key_mask.stride(0)
-    sdo = _NO_STRIDE if dout is None else _attn_tensor(dout, "dout", q.shape, dt, dev)[1]
-    sg = [_NO_STRIDE if g is None else _attn_tensor(g, n, t.shape, dt, dev)[1]
-          for g, n, t in zip(grads, ("dq", "dk", "dv"), (q, k, v))]
-    return _ATTN_SHAPE.pack(B, Hq, Hkv, Nq, Nk, D, 1 if causal else 0, code, ms, *sq, *sk, *sv, *so,
-                            *sdo, *sg[0], *sg[1], *sg[2], scale), key_mask
+    return key_mask, scale
+
+
+def _attn_shape(q, k, v, out, mask, causal, scale, dout=None, dq=None, dk=None, dv=None):
+    """The call's tts_attention_shape."""
+    B, Hq, Nq, D = q.shape
+    sg = [x for t in (dout, dq, dk, dv) for x in (_NO_STRIDE if t is None else _attn_stride(t))]
+    return _ATTN_SHAPE.pack(B, Hq, k.shape[1], Nq, k.shape[2], D, 1 if causal else 0,
+                            DTYPE_CODES[q.dtype], 0 if mask is None else mask.stride(0),
+                            *_attn_stride(q), *_attn_stride(k), *_attn_stride(v),
+                            *_attn_stride(out), *sg, scale)
 
 
 def _attn_like(t):
@@ -1216,8 +1261,16 @@ def _attn_like(t):
 
 
 def _attn_workspace(shape, backward, device):
-    n = _lib.load().tts_attention_workspace_bytes(shape, backward)
+    n = _size("tts_attention_workspace_bytes", shape, backward)
     return (torch.empty(n, device=device, dtype=U8), n) if n else (None, 0)
+
+
+def _attention_fwd(q, k, v, mask, causal, scale, out, lse):
+    shape = _attn_shape(q, k, v, out, mask, causal, scale)
+    ws, n = _attn_workspace(shape, 0, q.device)
+    _entry("tts_attention_fwd")(shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(mask),
+                                out.data_ptr(), _at(lse), _at(ws), n, _lib.raw_stream())
+    return out
 
 
 def attention_fwd(q, k, v, key_mask=None, causal=False, scale=None, out=None, lse=None):
@@ -1225,24 +1278,16 @@ def attention_fwd(q, k, v, key_mask=None, causal=False, scale=None, out=None, ls
     visible) and causal (row i sees keys up to i + Nk - Nq) leave; rows without a key give zeros.
     q [B, Hq, Nq, D], k and v [B, Hkv, Nk, D], Hq a multiple of Hkv, any strides with a contiguous
     last axis.  lse [B, Hq, Nq] fp32, when given, takes each row's log-sum-exp."""
-    out = _attn_like(q) if out is None else out
-    shape, mask = _attn_args(q, k, v, key_mask, causal, scale, out)
+    mask, scale = _attn_check(q, k, v, key_mask, scale, out)
     if lse is not None:
         require(lse, "lse", F32, q.shape[:3], q.device)
-    ws, n = _attn_workspace(shape, 0, q.device)
-    call("tts_attention_fwd", shape, ptr(q), ptr(k), ptr(v), ptr(mask), ptr(out), ptr(lse), ptr(ws),
-         n, stream())
-    return out
+    return _attention_fwd(q, k, v, mask, causal, scale, _attn_like(q) if out is None else out, lse)
 
 
-def attention_bwd(q, k, v, out, lse, dout, key_mask=None, causal=False, scale=None, need_dq=True,
-                  need_dk=True, need_dv=True):
-    """(dq, dk, dv) from the forward's out and lse; a part that is not needed is None."""
+def _attention_bwd(q, k, v, mask, causal, scale, out, lse, dout, need_dq, need_dk, need_dv):
     dq = _attn_like(q) if need_dq else None
     dk = _attn_like(k) if need_dk else None
     dv = _attn_like(v) if need_dv else None
-    shape, mask = _attn_args(q, k, v, key_mask, causal, scale, out, dout, (dq, dk, dv))
-    require(lse, "lse", F32, q.shape[:3], q.device)
     if not (need_dq or need_dk or need_dv):
         return None, None, None
     if q.shape[0] * q.shape[2] * k.shape[2] == 0:      # no score: no gradient
@@ -1250,7 +1295,18 @@ def attention_bwd(q, k, v, out, lse, dout, key_mask=None, causal=False, scale=No
             if g is not None:
                 g.zero_()
         return dq, dk, dv
+    shape = _attn_shape(q, k, v, out, mask, causal, scale, dout, dq, dk, dv)
     ws, n = _attn_workspace(shape, 1, q.device)
-    call("tts_attention_bwd", shape, ptr(q), ptr(k), ptr(v), ptr(mask), ptr(out), ptr(lse),
-         ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(ws), n, stream())
+    _entry("tts_attention_bwd")(shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(mask),
+                                out.data_ptr(), lse.data_ptr(), dout.data_ptr(), _at(dq), _at(dk),
+                                _at(dv), _at(ws), n, _lib.raw_stream())
     return dq, dk, dv
+
+
+def attention_bwd(q, k, v, out, lse, dout, key_mask=None, causal=False, scale=None, need_dq=True,
+                  need_dk=True, need_dv=True):
+    """(dq, dk, dv) from the forward's out and lse; a part that is not needed is None."""
+    mask, scale = _attn_check(q, k, v, key_mask, scale, out)
+    _attn_tensor(dout, "dout", q.shape, q.dtype, q.device)
+    require(lse, "lse", F32, q.shape[:3], q.device)
+    return _attention_bwd(q, k, v, mask, causal, scale, out, lse, dout, need_dq, need_dk, need_dv)

@@ -5,7 +5,6 @@ fp32, fp16 or bf16, weights of the same type or fp32; statistics and sums are fp
 gradients of weight and bias are summed over the rows in a fixed order.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels
 
@@ -26,17 +25,16 @@ class _LayerNorm(torch.autograd.Function):
         stats = torch.empty(rows.shape[0], 2, device=x.device, dtype=F32)
         y = kernels.layer_norm_fwd(rows, weight, bias, eps, stats=stats)
         ctx.save_for_backward(x, weight, stats)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return y.view(x.shape)
+        ctx.w_dtype = (bias.dtype if bias is not None else x.dtype) if weight is None else weight.dtype
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         nx, nw, nb, _ = ctx.needs_input_grad
-        dx, dw, db = kernels.layer_norm_bwd(_rows(x), weight, _rows(dy), stats, nx, nw, nb,
-                                            ctx.bias_dtype)
-        return (None if dx is None else dx.view(x.shape)), dw, db, None
+        dx, dw, db = kernels._layer_norm_bwd(_rows(x), weight, _rows(dy), stats, nx, nw, nb,
+                                             ctx.w_dtype)
+        return (dx if dx is None or x.dim() == 2 else dx.view(x.shape)), dw, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
