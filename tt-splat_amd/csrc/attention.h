@@ -61,6 +61,7 @@ struct AttnArgs {
   int64_t mask_stride;
   AttnStride sq, sk, sv, so, sdo, sdq, sdk, sdv;
   int Hkv, grp, Nq, Nk, D, R;   // R = Nq * grp rows a (batch, key head)
+  int D4;                       // D rounded up to 4: row stride of the parts of a split axis
   unsigned grp_mul;             // r / grp = (4 r * grp_mul >> 32) >> grp_shift for r < 2^30
   int grp_shift;
   int causal, off;              // row at position p sees keys up to p + off
@@ -358,7 +359,57 @@ __device__ __forceinline__ void store_column(T* row, int D, int db, const Acc& x
   }
 }
 
+// Joins the parts of split rows, in order: G groups of L lanes a row, each of which takes every G-th
+// part; the groups' sums are joined in a tree.  x: four columns' sum from column c on.  lse (softmax
+// parts): the parts' log-sum-exps weigh them, *m and *l are the maximum and the weights' sum.
+struct JoinTeam {
+  int lig, g, L, G;
+  int64_t row;
+  __device__ __forceinline__ JoinTeam(int L_, int G_)
+      : lig(threadIdx.x & (L_ - 1)), g(threadIdx.x / L_ & (G_ - 1)), L(L_), G(G_),
+        row((int64_t)blockIdx.x * (256 / (L_ * G_)) + threadIdx.x / (L_ * G_)) {}
+};
+__device__ __forceinline__ float join_max(const JoinTeam& t, const float* lse, int64_t rows,
+                                          int nsplit) {
+  float m = -INFINITY;
+  for (int s = t.g * t.L + t.lig; s < nsplit; s += t.L * t.G) m = fmaxf(m, lse[s * rows + t.row]);
+  for (int o = 1; o < t.L * t.G; o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
+  return m;
+}
+template <bool SOFT>
+__device__ __forceinline__ void join_parts(const JoinTeam& t, const float* part, const float* lse,
+                                           int64_t rows, int nsplit, int D4, int c, float m,
+                                           float* l, float (&x)[4]) {
+  *l = 0.0f;
+  x[0] = x[1] = x[2] = x[3] = 0.0f;
+#pragma unroll 4
+  for (int s = t.g; s < nsplit; s += t.G) {
+    const int64_t i = s * rows + t.row;
+    const float4 v = *reinterpret_cast<const float4*>(part + i * D4 + (c < D4 ? c : 0));
+    const float w = SOFT ? exp2_((lse[i] - m) * kLog2e) : 1.0f;
+    *l += w;
+    x[0] += w * v.x;
+    x[1] += w * v.y;
+    x[2] += w * v.z;
+    x[3] += w * v.w;
+  }
+  for (int o = t.L; o < t.L * t.G; o *= 2) {
+    *l += __shfl_xor(*l, o, 64);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] += __shfl_xor(x[j], o, 64);
+  }
+}
+
 // ---- host side ----
+
+// Lanes a row's columns and groups a row of a join over `nsplit` parts: groups while the rows alone
+// leave the card unfilled (256k threads; 40 000 rows of two parts with two groups 13 us, with one 8.5).
+inline void join_shape(int64_t rows, int D, int nsplit, int* L, int* G) {
+  *L = row_lanes((D + 3) / 4);
+  *G = 1;
+  while (*G * 2 <= nsplit && *L * *G < 64 && rows * *L * *G < (1 << 18)) *G *= 2;
+}
+inline int join_blocks(int64_t rows, int L, int G) { return (int)((rows * L * G + 255) / 256); }
 
 // Head sizes are rounded up to a multiple of 32; those that are no multiple of eight, to 32 or 128.
 template <typename F>
@@ -385,16 +436,14 @@ inline int launch_lds(K kernel, LdsLimit& lim, int blocks, int threads, size_t l
   return launch_status();
 }
 
-constexpr int kAttnFillBlocks = 512;   // two blocks a CU: below this the long axis is split
 constexpr int kAttnMaxSplit = 64;
 
-// Parts of `tiles` steps of the long axis for `blocks` blocks: as many as fill the card, each of
-// `least` steps or more.
-inline int attn_splits(int64_t blocks, int tiles, int least) {
-  if (blocks <= 0 || tiles <= 0) return 1;
-  int64_t n = kAttnFillBlocks / blocks;
-  const int64_t most = tiles / least;
-  n = n < most ? n : most;
+// Parts of `tiles` steps of the long axis for `waves` waves of work: as many as bring them nearest to
+// `fill`, each of `least` steps or more.
+inline int attn_splits(int64_t waves, int64_t fill, int tiles, int least) {
+  if (waves <= 0) return 1;
+  int64_t n = (fill + waves / 2) / waves;
+  n = n < tiles / least ? n : tiles / least;
   n = n < kAttnMaxSplit ? n : kAttnMaxSplit;
   return (int)(n < 1 ? 1 : n);
 }
@@ -406,7 +455,7 @@ struct AttnPlan {
   int kw, ks;        // dk, dv
   int rb_f, rb_q, kb;
 };
-AttnPlan attn_plan(const AttnArgs& a, int BH);
+AttnPlan attn_plan(const AttnArgs& a, int BH, int dtype);
 
 int attn_launch_fwd(const AttnArgs& a, int BH, int dtype, const AttnPlan& p, hipStream_t stream);
 int attn_launch_dq(const AttnArgs& a, int BH, int dtype, const AttnPlan& p, hipStream_t stream);

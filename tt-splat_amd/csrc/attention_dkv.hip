@@ -10,7 +10,6 @@
 // k_attn_dkv_join adds the parts in order.
 
 #include "attention.h"
-#include <cstdlib>
 
 namespace tts {
 
@@ -184,35 +183,29 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void k
     const int64_t i = (((int64_t)sp * (gridDim.x / nkb / a.nsplit) + bh) * a.Nk + key) * 2;
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
-      store_column(a.part2 + i * a.D, a.D, d, dk[d], a.scale);
-      store_column(a.part2 + (i + 1) * a.D, a.D, d, dv[d], 1.0f);
+      store_column(a.part2 + i * a.D4, a.D4, d, dk[d], a.scale);
+      store_column(a.part2 + (i + 1) * a.D4, a.D4, d, dv[d], 1.0f);
     }
   }
 }
 
-// Sums the parts of split keys, in order: L lanes a (key, dk or dv).
+// Sums the parts of split keys; a row is a (key, dk or dv).
 template <typename T>
-__global__ __launch_bounds__(256) void k_attn_dkv_join(AttnArgs a, int BH, int L) {
-  const int lig = threadIdx.x & (L - 1);
+__global__ __launch_bounds__(256) void k_attn_dkv_join(AttnArgs a, int BH, int L, int G) {
+  const JoinTeam t(L, G);
   const int64_t rows = (int64_t)BH * a.Nk * 2;
-  const int64_t i = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (i >= rows) return;
-  const int bh = (int)(i / 2 / a.Nk), key = (int)(i / 2 - (int64_t)bh * a.Nk);
+  if (t.row >= rows) return;
+  const int bh = (int)(t.row / 2 / a.Nk), key = (int)(t.row / 2 - (int64_t)bh * a.Nk);
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
-  const AttnStride& s = i & 1 ? a.sdv : a.sdk;
-  T* op = static_cast<T*>(i & 1 ? a.dv : a.dk);
+  const AttnStride& s = t.row & 1 ? a.sdv : a.sdk;
+  T* op = static_cast<T*>(t.row & 1 ? a.dv : a.dk);
   if (!op) return;
   op += b * s.b + hk * s.h + (int64_t)key * s.n;
-  for (int c = lig * 4; c < a.D; c += L * 4) {
-    float x[4] = {};
-#pragma unroll 4
-    for (int p = 0; p < a.nsplit; ++p) {
-      float v[4];
-      load_row(a.part2 + (p * rows + i) * a.D + c, a.D - c, v);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] += v[j];
-    }
-    store4(op + c, a.D - c, x[0], x[1], x[2], x[3]);
+  for (int c0 = 0; c0 < a.D; c0 += L * 4) {
+    const int c = c0 + t.lig * 4;
+    float x[4], l;
+    join_parts<false>(t, a.part2, nullptr, rows, a.nsplit, a.D4, c, 0.0f, &l, x);
+    if (t.g == 0) store4(op + c, a.D - c, x[0], x[1], x[2], x[3]);
   }
 }
 
@@ -238,35 +231,42 @@ int attn_launch_dkv(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hi
       return launch_dkv<T, dp(), 4, kDkvRows, odd()>(a, blocks, stream);
     });
     if (e || p.ks == 1) return e;
-    const int L = row_lanes((a.D + 3) / 4);
-    const int64_t rows = (int64_t)BH * a.Nk * 2;
-    k_attn_dkv_join<T><<<(int)((rows * L + 255) / 256), 256, 0, stream>>>(a, BH, L);
+    int L, G;
+    join_shape((int64_t)BH * a.Nk * 2, a.D, a.nsplit, &L, &G);
+    k_attn_dkv_join<T><<<join_blocks((int64_t)BH * a.Nk * 2, L, G), 256, 0, stream>>>(a, BH, L, G);
     return launch_status();
   });
 }
 
 // Up to 32 rows (keys) one wave a block holds them all; past that four waves share the tiles they
-// read.  Then the long axis is split until the card is full.
-AttnPlan attn_plan(const AttnArgs& a, int BH) {
+// read.  Half types with head sizes up to 64 give a wave 64 rows in the forward once that leaves a wave
+// for every second SIMD: each fragment of K and V then feeds two products (2500 x 2500, 16 heads of
+// 64: 77 -> 62 us with its join; 128 values a head leave it one wave a SIMD, 735 -> 810).  Then the
+// long axis is split until the waves that have work fill the card, two a SIMD: one where the keys'
+// kernel needs a SIMD's registers for itself.
+AttnPlan attn_plan(const AttnArgs& a, int BH, int dtype) {
   AttnPlan p;
-  p.fw = p.qw = a.R <= 32 && a.D % 8 == 0 ? 1 : 4;
-  const int bn = p.fw == 1 ? 32 : 64, tiles = (a.Nk - 1) / bn + 1;
-  p.fq = getenv("FQ2") && p.fw == 4 ? 2 : 1;
-  p.rb_q = (a.R - 1) / (32 * p.fw) + 1;
+  const bool odd = a.D % 8 != 0;
+  const int64_t row_waves = (int64_t)((a.R - 1) / 32 + 1) * BH;
+  const int64_t key_waves = (int64_t)((a.Nk - 1) / 32 + 1) * BH;
+  p.fw = p.qw = a.R <= 32 && !odd ? 1 : 4;
+  p.fq = p.fw == 4 && !odd && dtype != TTS_F32 && a.D <= 64 && row_waves >= 1024 ? 2 : 1;
   p.rb_f = (a.R - 1) / (32 * p.fw * p.fq) + 1;
-  p.fs = p.qs = attn_splits((int64_t)p.rb_f * BH, tiles, p.fw == 1 ? 2 : 4);
-  p.kw = a.Nk <= 32 && a.D % 8 == 0 ? 1 : 4;
+  p.rb_q = (a.R - 1) / (32 * p.qw) + 1;
+  const int tiles = (a.Nk - 1) / (p.fw == 1 ? 32 : 64) + 1;
+  p.fs = attn_splits(row_waves / p.fq, 2048, tiles, p.fw == 1 ? 2 : 4);
+  p.qs = attn_splits(row_waves, 2048, tiles, p.qw == 1 ? 2 : 4);
+  p.kw = a.Nk <= 32 && !odd ? 1 : 4;
   p.kb = (a.Nk - 1) / (32 * p.kw) + 1;
-  p.ks = attn_splits((int64_t)p.kb * BH, (a.R - 1) / (p.kw == 1 ? 32 : kDkvRows) + 1, 2);
-  auto ev = [](const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; };
-  p.fs = ev("FS", p.fs); p.qs = ev("QS", p.qs); p.ks = ev("KS", p.ks);
+  p.ks = attn_splits(key_waves, a.D <= 64 ? 2048 : 1024, (a.R - 1) / (p.kw == 1 ? 32 : kDkvRows) + 1,
+                     2);
   return p;
 }
 
 // Sub-buffers of the workspaces: forward's parts; backward's D, then parts of dQ and of dK, dV.
 size_t attn_fwd_layout(AttnArgs& a, int64_t BH, const AttnPlan& p, char* base) {
   if (p.fs == 1) return 0;
-  const size_t o = align256((size_t)p.fs * BH * a.R * a.D * sizeof(float));
+  const size_t o = align256((size_t)p.fs * BH * a.R * a.D4 * sizeof(float));
   a.part = reinterpret_cast<float*>(base);
   a.part2 = reinterpret_cast<float*>(base + o);
   return o + align256((size_t)p.fs * BH * a.R * sizeof(float));
@@ -279,8 +279,8 @@ size_t attn_bwd_layout(AttnArgs& a, int64_t BH, const AttnPlan& p, char* base) {
     return reinterpret_cast<float*>(r);
   };
   a.delta = take((size_t)BH * a.R * sizeof(float));
-  a.part = take(p.qs > 1 ? (size_t)p.qs * BH * a.R * a.D * sizeof(float) : 0);
-  a.part2 = take(p.ks > 1 ? (size_t)p.ks * BH * a.Nk * 2 * a.D * sizeof(float) : 0);
+  a.part = take(p.qs > 1 ? (size_t)p.qs * BH * a.R * a.D4 * sizeof(float) : 0);
+  a.part2 = take(p.ks > 1 ? (size_t)p.ks * BH * a.Nk * 2 * a.D4 * sizeof(float) : 0);
   return off;
 }
 
@@ -313,6 +313,7 @@ int attn_shape(const tts_attention_shape* s, AttnArgs* a, int* BH) {
   a->Nq = (int)s->queries;
   a->Nk = (int)s->keys;
   a->D = (int)s->head_dim;
+  a->D4 = (a->D + 3) & ~3;
   a->R = (int)(s->queries * grp);
   while ((1 << a->grp_shift) < grp) ++a->grp_shift;
   a->grp_mul = (unsigned)((((uint64_t)1 << (30 + a->grp_shift)) + grp - 1) / grp);
@@ -340,7 +341,7 @@ size_t tts_attention_workspace_bytes(const tts_attention_shape* shape, int backw
   AttnArgs a;
   int BH;
   if (!shape || attn_shape(shape, &a, &BH) || !BH || !a.R || !a.Nk) return 0;
-  const AttnPlan p = attn_plan(a, BH);
+  const AttnPlan p = attn_plan(a, BH, (int)shape->dtype);
   return backward ? attn_bwd_layout(a, BH, p, nullptr) : attn_fwd_layout(a, BH, p, nullptr);
 }
 
@@ -355,7 +356,7 @@ int tts_attention_fwd(const tts_attention_shape* shape, const void* q, const voi
   if (!q || !out || (a.Nk > 0 && (!k || !v))) return TTS_EINVAL;
   AttnPlan p = {};
   if (a.Nk > 0) {
-    p = attn_plan(a, BH);
+    p = attn_plan(a, BH, (int)shape->dtype);
   } else {   // no keys: rows of zeros, no tile is read
     p.fw = 4;
     p.rb_f = (a.R - 1) / 128 + 1;
@@ -385,7 +386,7 @@ int tts_attention_bwd(const tts_attention_shape* shape, const void* q, const voi
   if (const int e = attn_shape(shape, &a, &BH)) return e;
   if (!BH || !a.R || !a.Nk) return TTS_EINVAL;   // no product to differentiate
   if (!q || !k || !v || !out || !lse || !dout || (!dq && !dk && !dv)) return TTS_EINVAL;
-  const AttnPlan p = attn_plan(a, BH);
+  const AttnPlan p = attn_plan(a, BH, (int)shape->dtype);
   if (!attn_fits(a, BH, p)) return TTS_ELENGTH;
   a.q = q;
   a.k = k;

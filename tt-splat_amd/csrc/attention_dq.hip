@@ -152,31 +152,26 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
   } else {
     const int64_t i = ((int64_t)sp * (gridDim.x / nrb / a.nsplit) + bh) * a.R + row;
 #pragma unroll
-    for (int d = 0; d < DB; ++d) store_column(a.part + i * a.D, a.D, d, dq[d], a.scale);
+    for (int d = 0; d < DB; ++d) store_column(a.part + i * a.D4, a.D4, d, dq[d], a.scale);
   }
 }
 
-// Sums the parts of split rows, in order.
+// Sums the parts of split rows.
 template <typename T>
-__global__ __launch_bounds__(256) void k_attn_dq_join(AttnArgs a, int BH, int L) {
-  const int lig = threadIdx.x & (L - 1);
-  const int64_t rows = (int64_t)BH * a.R, i = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (i >= rows) return;
-  const int bh = (int)(i / a.R), row = (int)(i - (int64_t)bh * a.R);
+__global__ __launch_bounds__(256) void k_attn_dq_join(AttnArgs a, int BH, int L, int G) {
+  const JoinTeam t(L, G);
+  const int64_t rows = (int64_t)BH * a.R;
+  if (t.row >= rows) return;
+  const int bh = (int)(t.row / a.R), row = (int)(t.row - (int64_t)bh * a.R);
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   int pos, h;
   attn_row(a, row, &pos, &h);
   T* op = static_cast<T*>(a.dq) + b * a.sdq.b + (hk * a.grp + h) * a.sdq.h + (int64_t)pos * a.sdq.n;
-  for (int c = lig * 4; c < a.D; c += L * 4) {
-    float x[4] = {};
-#pragma unroll 4
-    for (int s = 0; s < a.nsplit; ++s) {
-      float v[4];
-      load_row(a.part + (s * rows + i) * a.D + c, a.D - c, v);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] += v[j];
-    }
-    store4(op + c, a.D - c, x[0], x[1], x[2], x[3]);
+  for (int c0 = 0; c0 < a.D; c0 += L * 4) {
+    const int c = c0 + t.lig * 4;
+    float x[4], l;
+    join_parts<false>(t, a.part, nullptr, rows, a.nsplit, a.D4, c, 0.0f, &l, x);
+    if (t.g == 0) store4(op + c, a.D - c, x[0], x[1], x[2], x[3]);
   }
 }
 
@@ -198,9 +193,9 @@ int attn_launch_dq(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hip
       return launch_dq<T, dp(), 4, 64, odd()>(a, blocks, stream);
     });
     if (e || p.qs == 1 || !a.dq) return e;
-    const int L = row_lanes((a.D + 3) / 4);
-    const int64_t rows = (int64_t)BH * a.R;
-    k_attn_dq_join<T><<<(int)((rows * L + 255) / 256), 256, 0, stream>>>(a, BH, L);
+    int L, G;
+    join_shape((int64_t)BH * a.R, a.D, a.nsplit, &L, &G);
+    k_attn_dq_join<T><<<join_blocks((int64_t)BH * a.R, L, G), 256, 0, stream>>>(a, BH, L, G);
     return launch_status();
   });
 }

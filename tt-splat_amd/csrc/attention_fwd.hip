@@ -1,6 +1,6 @@
 // Attention forward: one pass over the keys with the running maximum and sum of each row's softmax.
 //
-// A wave owns 32 rows (columns of S^T and O^T): Q stays in registers as the B operand, K and V tiles
+// A wave owns 32 QB rows (columns of S^T and O^T): Q stays in registers as the B operand, K and V tiles
 // of BN keys pass through LDS, read by all waves of the block, the next tile's loads in flight
 // while this one is computed.  Rows' maxima and sums are over a lane's own values; the two halves of
 // the wave are joined once a tile (maximum) and once at the end (sum).
@@ -21,7 +21,7 @@ constexpr size_t fwd_lds() {
 }
 
 template <typename T, int DP, int NW, int BN, int QB, bool ODD>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) && QB * DP <= 128 ? 2 : 1)
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2 : 1)
 void k_attn_fwd(AttnArgs a) {
   constexpr int KC = DP / 16, DB = DP / 32, KB = BN / 32, NT = 64 * NW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -211,45 +211,36 @@ void k_attn_fwd(AttnArgs a) {
     } else {
       const int64_t i = ((int64_t)sp * (gridDim.x / nrb / a.nsplit) + bh) * a.R + row;
 #pragma unroll
-      for (int d = 0; d < DB; ++d) store_column(a.part + i * a.D, a.D, d, o[j][d], inv);
+      for (int d = 0; d < DB; ++d) store_column(a.part + i * a.D4, a.D4, d, o[j][d], inv);
       if (hi == 0) a.part2[i] = lse;
     }
   }
 }
 
-// Joins the parts of split rows: L lanes a row, parts in order.
+// Joins the parts of split rows.
 template <typename T>
-__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int BH, int L) {
-  const int lig = threadIdx.x & (L - 1);
-  const int64_t rows = (int64_t)BH * a.R, i = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (i >= rows) return;
-  const int bh = (int)(i / a.R), row = (int)(i - (int64_t)bh * a.R);
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int BH, int L, int G) {
+  const JoinTeam t(L, G);
+  const int64_t rows = (int64_t)BH * a.R;
+  if (t.row >= rows) return;
+  const int bh = (int)(t.row / a.R), row = (int)(t.row - (int64_t)bh * a.R);
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   int pos, h;
   attn_row(a, row, &pos, &h);
   const int hq = hk * a.grp + h;
-  float m = -INFINITY, l = 0.0f;
-  for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.part2[s * rows + i]);
-  const float base = m == -INFINITY ? 0.0f : m;
-  // a NaN in any part reaches the sum, as it does in one pass
-  for (int s = 0; s < a.nsplit; ++s) l += exp2_((a.part2[s * rows + i] - base) * kLog2e);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float mx = join_max(t, a.part2, rows, a.nsplit), m = mx == -INFINITY ? 0.0f : mx;
   T* op = static_cast<T*>(a.out) + b * a.so.b + hq * a.so.h + (int64_t)pos * a.so.n;
-  for (int c = lig * 4; c < a.D; c += L * 4) {
-    float x[4] = {};
-#pragma unroll 4
-    for (int s = 0; s < a.nsplit; ++s) {
-      const float w = exp2_((a.part2[s * rows + i] - base) * kLog2e);
-      float v[4];
-      load_row(a.part + (s * rows + i) * a.D + c, a.D - c, v);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] += w * v[j];
-    }
-    store4(op + c, a.D - c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  float l = 0.0f;
+  for (int c0 = 0; c0 < a.D; c0 += L * 4) {
+    const int c = c0 + t.lig * 4;
+    float x[4];
+    join_parts<true>(t, a.part, a.part2, rows, a.nsplit, a.D4, c, m, &l, x);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (t.g == 0) store4(op + c, a.D - c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
   }
-  if (a.lse && lig == 0)
+  if (a.lse && t.g == 0 && t.lig == 0)
     a.lse[((int64_t)b * a.Hkv * a.grp + hq) * a.Nq + pos] =
-        l == 0.0f ? -INFINITY : base + kLn2 * __log2f(l);
+        l == 0.0f ? -INFINITY : m + kLn2 * __log2f(l);
 }
 
 template <typename T, int DP, int NW, int BN, int QB, bool ODD>
@@ -268,14 +259,14 @@ int attn_launch_fwd(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hi
     const int e = by_head(a.D, [&](auto dp, auto odd) {
       if constexpr (!odd())
         if (p.fw == 1) return launch_fwd<T, dp(), 1, 32, 1, false>(a, blocks, stream);
-      if constexpr (!odd() && sizeof(T) == 2)
+      if constexpr (!odd() && sizeof(T) == 2 && dp() <= 64)
         if (p.fq == 2) return launch_fwd<T, dp(), 4, 64, 2, false>(a, blocks, stream);
       return launch_fwd<T, dp(), 4, 64, 1, odd()>(a, blocks, stream);
     });
     if (e || p.fs == 1) return e;
-    const int L = row_lanes((a.D + 3) / 4);
-    const int64_t rows = (int64_t)BH * a.R;
-    k_attn_join<T><<<(int)((rows * L + 255) / 256), 256, 0, stream>>>(a, BH, L);
+    int L, G;
+    join_shape((int64_t)BH * a.R, a.D, a.nsplit, &L, &G);
+    k_attn_join<T><<<join_blocks((int64_t)BH * a.R, L, G), 256, 0, stream>>>(a, BH, L, G);
     return launch_status();
   });
 }
