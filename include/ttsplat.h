@@ -668,17 +668,18 @@ size_t tts_attention_workspace_bytes(const tts_attention_shape* shape, int backw
 
 /* out = softmax(scale q k^T over the visible keys) v.  key_mask (may be NULL): one byte for each batch
  * and key, 0 hides the key, whose k and v rows may hold anything.  A row that sees no key gives zeros.
+ * rest (may be NULL; half types): what rounding out left behind, of out's strides, for the backward.
  * lse [batch, heads, queries] fp32 contiguous (may be NULL where no backward follows): the
  * log-sum-exp of each row's scores, -inf for a row without a key. */
 int tts_attention_fwd(const tts_attention_shape* shape, const void* q, const void* k,
-                      const void* v, const uint8_t* key_mask, void* out, float* lse,
+                      const void* v, const uint8_t* key_mask, void* out, void* rest, float* lse,
                       void* workspace, size_t workspace_bytes, hipStream_t stream);
 
-/* Its gradients, from out and lse (the probabilities are recomputed): dq, dk, dv, each may be NULL (not
+/* Its gradients, from out, rest (may be NULL) and lse (the probabilities are recomputed): dq, dk, dv, each may be NULL (not
  * all).  Hidden keys get zeros.  Deterministic: no atomics.  Sizes of zero are refused. */
 int tts_attention_bwd(const tts_attention_shape* shape, const void* q, const void* k,
-                      const void* v, const uint8_t* key_mask, const void* out, const float* lse,
-                      const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                      const void* v, const uint8_t* key_mask, const void* out, const void* rest,
+                      const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
                       size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus

@@ -295,5 +295,5 @@ def test_refusals():
     shape = kernels._attn_shape(q, k, v, q, None, False, 0.25, q, q, k, v)
     with pytest.raises(_lib.TTSError):       # no workspace
         _lib.call("tts_attention_bwd", shape, *(_lib.ptr(t) for t in (q, k, v)), None,
-                  _lib.ptr(q), _lib.ptr(q), _lib.ptr(q), _lib.ptr(q), None, None, None, 0,
+                  _lib.ptr(q), None, _lib.ptr(q), _lib.ptr(q), _lib.ptr(q), None, None, None, 0,
                   _lib.stream())

@@ -54,8 +54,8 @@ struct AttnStride {
 };
 
 struct AttnArgs {
-  const void *q, *k, *v, *o, *dout;
-  void *out, *dq, *dk, *dv;
+  const void *q, *k, *v, *o, *orest, *dout;
+  void *out, *rest, *dq, *dk, *dv;
   float *lse, *delta, *part, *part2;
   const uint8_t* mask;
   int64_t mask_stride;
@@ -398,6 +398,14 @@ __device__ __forceinline__ void join_parts(const JoinTeam& t, const float* part,
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] += __shfl_xor(x[j], o, 64);
   }
+}
+
+// What rounding the output left out: x - (T)x, and nothing where it is below the fp32 sums' own error
+// (a row with one key has O = V and no rest).
+template <typename T>
+__device__ __forceinline__ float rest_of(float x) {
+  const float r = x - (float)(T)x;
+  return fabsf(r) > fabsf(x) * 0x1p-20f ? r : 0.0f;
 }
 
 // ---- host side ----

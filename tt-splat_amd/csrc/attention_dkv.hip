@@ -346,7 +346,7 @@ size_t tts_attention_workspace_bytes(const tts_attention_shape* shape, int backw
 }
 
 int tts_attention_fwd(const tts_attention_shape* shape, const void* q, const void* k,
-                      const void* v, const uint8_t* key_mask, void* out, float* lse,
+                      const void* v, const uint8_t* key_mask, void* out, void* rest, float* lse,
                       void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (!shape) return TTS_EINVAL;
   AttnArgs a;
@@ -370,6 +370,7 @@ int tts_attention_fwd(const tts_attention_shape* shape, const void* q, const voi
   a.v = v;
   a.mask = key_mask;
   a.out = out;
+  a.rest = rest;
   a.lse = lse;
   const size_t need = attn_fwd_layout(a, BH, p, static_cast<char*>(workspace));
   if (need && (!workspace || workspace_bytes < need)) return TTS_EWORKSPACE;
@@ -377,8 +378,8 @@ int tts_attention_fwd(const tts_attention_shape* shape, const void* q, const voi
 }
 
 int tts_attention_bwd(const tts_attention_shape* shape, const void* q, const void* k,
-                      const void* v, const uint8_t* key_mask, const void* out, const float* lse,
-                      const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                      const void* v, const uint8_t* key_mask, const void* out, const void* rest,
+                      const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
                       size_t workspace_bytes, hipStream_t stream) {
   if (!shape) return TTS_EINVAL;
   AttnArgs a;
@@ -393,6 +394,7 @@ int tts_attention_bwd(const tts_attention_shape* shape, const void* q, const voi
   a.v = v;
   a.mask = key_mask;
   a.o = out;
+  a.orest = rest;
   a.lse = const_cast<float*>(lse);
   a.dout = dout;
   a.dq = dq;

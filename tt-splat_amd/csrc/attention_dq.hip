@@ -53,6 +53,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
       of[c] = load_frag(op + d, a.D - d);
     }
     delta = row_dots<T, KC>(of, go);
+    if (sizeof(T) == 2 && a.orest) {   // what O's rounding left out
+      const T* rp = static_cast<const T*>(a.orest) + (op - static_cast<const T*>(a.o));
+#pragma unroll
+      for (int c = 0; c < KC; ++c) of[c] = load_frag(rp + c * 16 + hi * 8, a.D - c * 16 - hi * 8);
+      delta += row_dots<T, KC>(of, go);
+    }
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
       arrive(q[c]);

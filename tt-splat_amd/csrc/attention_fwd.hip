@@ -8,6 +8,9 @@
 // Roundings: S, the softmax and O are fp32; P is rounded to the operands' type for its product with V
 // (half types), O once at the end.
 //
+// For a backward in half types the rounding's rest, O - (T)O, is stored beside O: D = rowsum(dO O) then
+// carries 16 bits of O, not 8 or 11 (without it dQ and dK of short key axes lose a quarter of a bit).
+//
 // Few rows (serving): one wave a block and the keys split over blocks; each part leaves its normalised
 // O and its log-sum-exp, and k_attn_join adds the parts by exp(L_part - L).
 
@@ -207,6 +210,16 @@ void k_attn_fwd(AttnArgs a) {
       T* op = static_cast<T*>(a.out) + b * a.so.b + hq * a.so.h + (int64_t)pos * a.so.n;
 #pragma unroll
       for (int d = 0; d < DB; ++d) store_column(op, a.D, d, o[j][d], inv);
+      if (sizeof(T) == 2 && a.rest) {
+        T* rp = static_cast<T*>(a.rest) + (op - static_cast<T*>(a.out));
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          Acc x;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = rest_of<T>(o[j][d][i] * inv);
+          store_column(rp, a.D, d, x, 1.0f);
+        }
+      }
       if (a.lse && hi == 0) a.lse[((int64_t)b * a.Hkv * a.grp + hq) * a.Nq + pos] = lse;
     } else {
       const int64_t i = ((int64_t)sp * (gridDim.x / nrb / a.nsplit) + bh) * a.R + row;
@@ -236,7 +249,14 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int BH, int L, in
     float x[4];
     join_parts<true>(t, a.part, a.part2, rows, a.nsplit, a.D4, c, m, &l, x);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (t.g == 0) store4(op + c, a.D - c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    if (t.g == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] *= inv;
+      store4(op + c, a.D - c, x[0], x[1], x[2], x[3]);
+      if (sizeof(T) == 2 && a.rest)
+        store4(static_cast<T*>(a.rest) + (op + c - static_cast<T*>(a.out)), a.D - c,
+               rest_of<T>(x[0]), rest_of<T>(x[1]), rest_of<T>(x[2]), rest_of<T>(x[3]));
+    }
   }
   if (a.lse && t.g == 0 && t.lig == 0)
     a.lse[((int64_t)b * a.Hkv * a.grp + hq) * a.Nq + pos] =

@@ -140,9 +140,9 @@ SIGNATURES = {
     "tts_embedding_bwd": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_i64, _c_int, _c_float, _c_int,
                                    _vp, _vp, _c_size, _vp]),
     "tts_attention_workspace_bytes": (_c_size, [_vp, _c_int]),
-    "tts_attention_fwd": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_size, _vp]),
+    "tts_attention_fwd": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_size, _vp]),
     "tts_attention_bwd": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
-                                   _c_size, _vp]),
+                                   _vp, _c_size, _vp]),
 }
 
 _lib = None

@@ -2,8 +2,9 @@
 among themselves.
 
 `attention(q, k, v, key_mask, causal, scale)` is differentiable w.r.t. q, k and v.  The forward
-keeps each row's log-sum-exp and no scores; the backward recomputes the probabilities.  Types
-fp32, fp16 and bf16; the softmax and all sums are fp32.  Results are the same bits every time.
+keeps no scores, but each row's log-sum-exp and, in half types, what rounding the output left
+behind; the backward recomputes the probabilities.  Types fp32, fp16 and bf16; the softmax and all
+sums are fp32.  Results are the same bits every time.
 """
 import torch
 
@@ -23,17 +24,19 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, causal, scale):
         lse = torch.empty(q.shape[:3], device=q.device, dtype=F32)
-        out = kernels._attention_fwd(q, k, v, mask, causal, scale, kernels._attn_like(q), lse)
-        ctx.save_for_backward(q, k, v, mask, out, lse)
+        out = kernels._attn_like(q)
+        rest = None if q.dtype == F32 else torch.empty_like(out)
+        kernels._attention_fwd(q, k, v, mask, causal, scale, out, lse, rest)
+        ctx.save_for_backward(q, k, v, mask, out, rest, lse)
         ctx.meta = (causal, scale)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, mask, out, lse = ctx.saved_tensors
+        q, k, v, mask, out, rest, lse = ctx.saved_tensors
         causal, scale = ctx.meta
         nq, nk, nv, _, _, _ = ctx.needs_input_grad
-        grads = kernels._attention_bwd(q, k, v, mask, causal, scale, out, lse,
+        grads = kernels._attention_bwd(q, k, v, mask, causal, scale, out, rest, lse,
                                        _last_contiguous(dout), nq, nk, nv)
         return (*grads, None, None, None)
 

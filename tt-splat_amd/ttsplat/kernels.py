@@ -1260,31 +1260,43 @@ def _attn_like(t):
         t.shape, device=t.device, dtype=t.dtype)
 
 
+def _attn_rest(rest, out):
+    if rest is not None:
+        _attn_tensor(rest, "rest", out.shape, out.dtype, out.device)
+        if rest.stride() != out.stride():
+            raise ValueError("rest must have the strides of out")
+
+
 def _attn_workspace(shape, backward, device):
     n = _size("tts_attention_workspace_bytes", shape, backward)
     return (torch.empty(n, device=device, dtype=U8), n) if n else (None, 0)
 
 
-def _attention_fwd(q, k, v, mask, causal, scale, out, lse):
+def _attention_fwd(q, k, v, mask, causal, scale, out, lse, rest=None):
     shape = _attn_shape(q, k, v, out, mask, causal, scale)
     ws, n = _attn_workspace(shape, 0, q.device)
     _entry("tts_attention_fwd")(shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(mask),
-                                out.data_ptr(), _at(lse), _at(ws), n, _lib.raw_stream())
+                                out.data_ptr(), _at(rest), _at(lse), _at(ws), n,
+                                _lib.raw_stream())
     return out
 
 
-def attention_fwd(q, k, v, key_mask=None, causal=False, scale=None, out=None, lse=None):
+def attention_fwd(q, k, v, key_mask=None, causal=False, scale=None, out=None, lse=None,
+                  rest=None):
     """out [B, Hq, Nq, D] = softmax(scale q k^T) v over the keys that key_mask [B, Nk] (non-zero:
     visible) and causal (row i sees keys up to i + Nk - Nq) leave; rows without a key give zeros.
     q [B, Hq, Nq, D], k and v [B, Hkv, Nk, D], Hq a multiple of Hkv, any strides with a contiguous
-    last axis.  lse [B, Hq, Nq] fp32, when given, takes each row's log-sum-exp."""
+    last axis.  For a backward: lse [B, Hq, Nq] fp32 takes each row's log-sum-exp; rest (half types,
+    out's shape and strides) what out's rounding left behind, which sharpens dq and dk."""
     mask, scale = _attn_check(q, k, v, key_mask, scale, out)
     if lse is not None:
         require(lse, "lse", F32, q.shape[:3], q.device)
-    return _attention_fwd(q, k, v, mask, causal, scale, _attn_like(q) if out is None else out, lse)
+    out = _attn_like(q) if out is None else out
+    _attn_rest(rest, out)
+    return _attention_fwd(q, k, v, mask, causal, scale, out, lse, rest)
 
 
-def _attention_bwd(q, k, v, mask, causal, scale, out, lse, dout, need_dq, need_dk, need_dv):
+def _attention_bwd(q, k, v, mask, causal, scale, out, rest, lse, dout, need_dq, need_dk, need_dv):
     dq = _attn_like(q) if need_dq else None
     dk = _attn_like(k) if need_dk else None
     dv = _attn_like(v) if need_dv else None
@@ -1298,15 +1310,17 @@ def _attention_bwd(q, k, v, mask, causal, scale, out, lse, dout, need_dq, need_d
     shape = _attn_shape(q, k, v, out, mask, causal, scale, dout, dq, dk, dv)
     ws, n = _attn_workspace(shape, 1, q.device)
     _entry("tts_attention_bwd")(shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(mask),
-                                out.data_ptr(), lse.data_ptr(), dout.data_ptr(), _at(dq), _at(dk),
-                                _at(dv), _at(ws), n, _lib.raw_stream())
+                                out.data_ptr(), _at(rest), lse.data_ptr(), dout.data_ptr(),
+                                _at(dq), _at(dk), _at(dv), _at(ws), n, _lib.raw_stream())
     return dq, dk, dv
 
 
 def attention_bwd(q, k, v, out, lse, dout, key_mask=None, causal=False, scale=None, need_dq=True,
-                  need_dk=True, need_dv=True):
-    """(dq, dk, dv) from the forward's out and lse; a part that is not needed is None."""
+                  need_dk=True, need_dv=True, rest=None):
+    """(dq, dk, dv) from the forward's out, lse and rest; a part that is not needed is None."""
     mask, scale = _attn_check(q, k, v, key_mask, scale, out)
     _attn_tensor(dout, "dout", q.shape, q.dtype, q.device)
     require(lse, "lse", F32, q.shape[:3], q.device)
-    return _attention_bwd(q, k, v, mask, causal, scale, out, lse, dout, need_dq, need_dk, need_dv)
+    _attn_rest(rest, out)
+    return _attention_bwd(q, k, v, mask, causal, scale, out, rest, lse, dout, need_dq, need_dk,
+                          need_dv)
