@@ -79,12 +79,18 @@ __device__ __forceinline__ int64_t row_offset(const AttnStride& s, int pos, int 
   return h * s.h + (int64_t)pos * s.n;
 }
 
+// Eight values at any element's address.
+template <typename T>
+__device__ __forceinline__ Frag<T> load_whole(const T* p) {
+  typedef int Any __attribute__((ext_vector_type(2 * sizeof(T)), aligned(sizeof(T))));
+  return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const Any*>(p));
+}
 // Eight values at p, n of them within the row, zeros behind.
 template <typename T>
 __device__ __forceinline__ Frag<T> load_frag(const T* p, int n) {
   Frag<T> f;
   if (n >= 8) {
-    memcpy(&f, p, 8 * sizeof(T));
+    f = load_whole(p);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = i < n ? p[i] : (T)0.0f;
@@ -96,29 +102,32 @@ __device__ __forceinline__ Frag<T> load_frag(const T* p, int n) {
 // be for every load that is in flight there, the next tile's among them.
 template <typename F>
 __device__ __forceinline__ void arrive(F& f) {
-  constexpr int N = sizeof(F) / 16;
-  using V4 = int __attribute__((ext_vector_type(4)));
-  V4 v[N];
-  memcpy(v, &f, sizeof(F));
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
-  memcpy(&f, v, sizeof(F));
+  asm volatile("" : "+v"(f));
 }
 
-// Tiles in LDS: row-major, rows longer than their data so that one read's lanes meet different banks
-// (64 of 4 bytes).  Half types: 32 bytes longer, a stride of 8 banks past a multiple of 16; a fragment's
-// 8 lanes a clock take 4 banks each of 8 rows, a transposed read's 16 lanes 8 banks each of 4 rows.
-// fp32: 16 bytes longer; transposed reads take 32 values of one row.
+// Tiles in LDS: row-major, rows longer than their data so that one read's lanes meet different banks.
+// Half types: 32 bytes longer: a transposed read's four rows of 32 bytes a clock are apart (115 of 128
+// bytes a clock and CU with four waves); a fragment's eight rows of 16 bytes meet in pairs, and pieces
+// exchanged within unpadded rows by an exclusive or, which part them too, measured the same in these
+// kernels (2500 x 2500: 236 -> 232 us for this form).  fp32: 16 bytes longer; transposed reads
+// take 32 values of one row.
 template <typename T, int DP>
 constexpr int kTileStride = DP + (sizeof(T) == 2 ? 16 : 4);
+
+using Piece = int __attribute__((ext_vector_type(4)));
+template <typename T>
+using Pieces = int __attribute__((ext_vector_type(2 * sizeof(T))));   // a fragment's, one or two
 
 template <typename T, int DP>
 __device__ __forceinline__ Frag<T> tile_frag(const T* tile, int row0, int d0) {
   const int lane = threadIdx.x & 63;
-  Frag<T> f;
-  memcpy(&f, __builtin_assume_aligned(tile + (row0 + (lane & 31)) * kTileStride<T, DP> + d0 +
-                                          (lane >> 5) * 8, 16), 8 * sizeof(T));
-  return f;
+  const T* p = tile + (row0 + (lane & 31)) * kTileStride<T, DP> + d0 + (lane >> 5) * 8;
+  if constexpr (sizeof(T) == 2) {
+    return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const Piece*>(p));
+  } else {
+    const Piece lo = *reinterpret_cast<const Piece*>(p), up = *reinterpret_cast<const Piece*>(p + 4);
+    return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
 }
 
 // A operand whose rows are the tile's columns d0 .. d0 + 31 and whose depth is its rows row0 ..
@@ -131,8 +140,8 @@ __device__ __forceinline__ Frag<T> transpose_frag(const T* tile, int row0, int d
     // lane l receives column l
     using S4 = short __attribute__((ext_vector_type(4)));
     using LdsPtr = __attribute__((address_space(3))) S4*;
-    const T* p = tile + (row0 + 4 * hi + ((lane & 15) >> 2)) * kTileStride<T, DP> + d0 +
-                 (lane & 16) + 4 * (lane & 3);
+    const T* p = tile + (row0 + 4 * hi + ((lane & 15) >> 2)) * kTileStride<T, DP> + d0 + (lane & 16) +
+                 4 * (lane & 3);
     const S4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)p);
     const S4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + 8 * kTileStride<T, DP>));
     const short __attribute__((ext_vector_type(8))) r =
@@ -176,7 +185,7 @@ struct TileLoad {
         get(i, first + n * stride, d0, D);
       } else {
         const unsigned off = (unsigned)(n * stride + (d0 < D ? d0 : 0)) * (unsigned)sizeof(T);
-        memcpy(&r[i], reinterpret_cast<const char*>(first) + off, 8 * sizeof(T));
+        r[i] = load_whole(reinterpret_cast<const T*>(reinterpret_cast<const char*>(first) + off));
       }
     }
   }
@@ -185,16 +194,15 @@ struct TileLoad {
 #pragma unroll
       for (int j = 0; j < 8; ++j) r[i][j] = p[d0 + j < D ? d0 + j : 0];
     } else {
-      memcpy(&r[i], p + (d0 < D ? d0 : 0), 8 * sizeof(T));
+      r[i] = load_whole(p + (d0 < D ? d0 : 0));
     }
   }
   __device__ __forceinline__ void store(T* tile, uint64_t live, int D) const {
-    constexpr int kWords = 2 * (int)sizeof(T);
     if (!ODD && D == DP && live == (BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1)) {
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
         const int v = threadIdx.x + i * NT;
-        memcpy(at(tile, v), &r[i], 8 * sizeof(T));
+        write(tile, v, __builtin_bit_cast(Pieces<T>, r[i]));
       }
       return;
     }
@@ -208,16 +216,19 @@ struct TileLoad {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = d0 + j < D ? f[j] : (T)0.0f;
       }
-      uint32_t w[kWords];
-      memcpy(w, &f, sizeof(f));
-#pragma unroll
-      for (int j = 0; j < kWords; ++j) w[j] = on ? w[j] : 0;
-      memcpy(at(tile, v), w, sizeof(f));
+      const Pieces<T> w = __builtin_bit_cast(Pieces<T>, f);
+      write(tile, v, on ? w : Pieces<T>{});
     }
   }
-  static __device__ __forceinline__ T* at(T* tile, int v) {
-    return static_cast<T*>(__builtin_assume_aligned(
-        tile + v / kPerRow * kTileStride<T, DP> + v % kPerRow * 8, 16));
+  // Whole pieces of 16 bytes: byte copies here are taken apart into byte stores by the compiler.
+  static __device__ __forceinline__ void write(T* tile, int v, Pieces<T> w) {
+    T* p = tile + v / kPerRow * kTileStride<T, DP> + v % kPerRow * 8;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<Piece*>(p) = w;
+    } else {
+      *reinterpret_cast<Piece*>(p) = __builtin_shufflevector(w, w, 0, 1, 2, 3);
+      *reinterpret_cast<Piece*>(p + 4) = __builtin_shufflevector(w, w, 4, 5, 6, 7);
+    }
   }
 };
 

@@ -228,7 +228,9 @@ int attn_launch_dkv(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hi
     const int e = by_head(a.D, [&](auto dp, auto odd) {
       if constexpr (!odd())
         if (p.kw == 1) return launch_dkv<T, dp(), 1, 32, false>(a, blocks, stream);
-      return launch_dkv<T, dp(), 4, kDkvRows, odd()>(a, blocks, stream);
+      // fp32 with 128 values a head: half the rows a tile, which leaves its registers unspilled
+      constexpr int kRows = sizeof(T) == 4 && dp() == 128 ? kDkvRows / 2 : kDkvRows;
+      return launch_dkv<T, dp(), 4, kRows, odd()>(a, blocks, stream);
     });
     if (e || p.ks == 1) return e;
     int L, G;
