@@ -175,6 +175,21 @@ def test_strides():
         check(q, k, v, do[:, :1, :1].expand(2, 4, 90, 24))
 
 
+def test_offsets_past_32_bits():
+    """Rows a million elements apart: the last ones lie 8 GB behind the first."""
+    q, k, v, do = inputs(1, 2, 2, 70, 2100, 32, torch.bfloat16)
+    wide = torch.empty(2100, 1 << 21, device="cuda", dtype=torch.bfloat16)   # 8.8 GB, written in part
+    views = []
+    for i, t in enumerate((k, v)):
+        w = wide[:, 4096 * i:4096 * i + 64].view(2100, 2, 32).permute(1, 0, 2)[None]
+        w.copy_(t)
+        views.append(w)
+    check(q, *views, do)
+    check(views[0], k[:, :, :90], v[:, :, :90], views[1])       # as query rows and their gradient
+    qg = torch.cat([views[0], views[1]], 1)                      # grouped heads over far rows
+    check(qg, k[:, :, :50], v[:, :, :50], qg.flip(2))
+
+
 def test_large_scores():
     """Scores of several hundred: the softmax is taken from each row's maximum; a row's largest few
     keys carry it, and the rest underflow to zero."""

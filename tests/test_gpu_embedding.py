@@ -122,6 +122,24 @@ def test_nothing():
     assert y.shape == (0, 6) and torch.equal(g, torch.zeros(4, 6, device="cuda"))
 
 
+def test_offsets_past_32_bits():
+    """A table of 5 GB: rows at its end, and their gradient."""
+    from ttsplat import kernels
+    V, D = 40_000_000, 64
+    table = torch.empty(V, D, device="cuda", dtype=torch.bfloat16)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    ids = torch.randint(V - 900, V, (3000,), device="cuda", generator=gen)
+    table[V - 900:] = torch.randn(900, D, device="cuda", generator=gen).to(torch.bfloat16)
+    dy = torch.randn(3000, D, device="cuda", generator=gen).to(torch.bfloat16)
+    assert torch.equal(kernels.embedding_fwd(table, ids), table[ids])
+    del table
+    g = kernels.embedding_bwd(dy, ids, V)
+    ref = torch.zeros(900, D, dtype=torch.float64).index_add_(0, (ids - (V - 900)).cpu(), dy.double().cpu())
+    err = (g[V - 900:].double().cpu() - ref).abs()
+    assert bool((err <= 2.0 ** -7 * ref.abs() + 1e-5 * 20).all())
+    assert int(g[:V - 900].count_nonzero()) == 0
+
+
 def test_rows_outside_leave_nan_out():
     """A NaN in the gradient of a token without an entry reaches no row."""
     table, ids, dy = inputs(200, 10, 8, torch.float32, "uniform")

@@ -113,6 +113,15 @@ def test_strides_and_shapes():
     check(x, dy[:1].expand(40, 96), w, b)
 
 
+def test_offsets_past_32_bits():
+    """Rows two million elements apart, the last 8 GB behind the first."""
+    wide = torch.empty(2100, 1 << 21, device="cuda", dtype=torch.bfloat16)
+    x, dy, w, b = inputs((2100, 40), torch.bfloat16, torch.float32)
+    wide[:, :40] = x
+    wide[:, 64:104] = dy
+    check(wide[:, :40], wide[:, 64:104], w, b)
+
+
 def test_no_rows():
     from ttsplat.norm import layer_norm
     x = torch.empty(0, 16, device="cuda", requires_grad=True)

@@ -65,6 +65,7 @@ struct AttnArgs {
   unsigned grp_mul;             // r / grp = (4 r * grp_mul >> 32) >> grp_shift for r < 2^30
   int grp_shift;
   int causal, off;              // row at position p sees keys up to p + off
+  int even_rows;                // tiles of 32 rows start at whole positions, their offsets are 32-bit
   int nsplit;                   // parts of the long axis, joined by a second kernel
   float scale;
 };
@@ -166,7 +167,22 @@ struct TileLoad {
   static constexpr int kPerRow = DP / 8, kN = BN * kPerRow / NT;
   static_assert(kN * NT == BN * kPerRow, "threads must divide the tile");
   Frag<T> r[kN];
+  unsigned off[kN];   // bytes from a whole tile's first row, the same for every tile
 
+  // at(i): elements from a whole tile's first row to its row i, below 2^31 bytes
+  template <typename At>
+  __device__ __forceinline__ void plan(int D, At at) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int v = threadIdx.x + i * NT, d0 = v % kPerRow * 8;
+      off[i] = (unsigned)(at(v / kPerRow) + (d0 < D ? d0 : 0)) * (unsigned)sizeof(T);
+    }
+  }
+  __device__ __forceinline__ void load_planned(const T* first) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      r[i] = load_whole(reinterpret_cast<const T*>(reinterpret_cast<const char*>(first) + off[i]));
+  }
   // row(i): pointer to the tile's row i (any valid row for rows that are not live)
   template <typename Row>
   __device__ __forceinline__ void load(int D, Row row) {

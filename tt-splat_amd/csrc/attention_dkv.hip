@@ -81,9 +81,44 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void k
   }
 
   TileLoad<T, DP, BM, NT, ODD> lq, lg;
+  // even rows: a whole tile's addresses are its first row's and offsets that are the same for every tile
+  // (half types: the offsets would push fp32 tiles of 128 values out of the registers)
+  constexpr bool kPlan = !ODD && sizeof(T) == 2;
+  int lse_off, lim_off;
+  if constexpr (kPlan) {
+    auto at = [&](const AttnStride& s) {
+      return [&](int n) {
+        int pos, h;
+        attn_row(a, n, &pos, &h);
+        return (int)(h * s.h) + pos * s.n;
+      };
+    };
+    if (a.even_rows) {
+      lq.plan(a.D, at(a.sq));
+      lg.plan(a.D, at(a.sdo));
+    }
+  }
+  {
+    int pos, h;
+    attn_row(a, threadIdx.x & (BM - 1), &pos, &h);
+    lse_off = h * a.Nq + pos;   // below R, which is below 2^30
+    lim_off = pos + a.off;
+  }
+  const float* lsep = a.lse + (int64_t)bh * a.grp * a.Nq;
   float st0 = 0.0f, st1 = 0.0f;
   int st2 = 0;
   auto fetch = [&](int tile) {
+    if (kPlan && a.even_rows && (tile + 1) * BM <= a.R) {
+      int pos0, h0;
+      attn_row(a, tile * BM, &pos0, &h0);
+      pos0 = __builtin_amdgcn_readfirstlane(pos0);
+      lq.load_planned(qp + (int64_t)pos0 * a.sq.n);
+      lg.load_planned(gp + (int64_t)pos0 * a.sdo.n);
+      st0 = lsep[pos0 + lse_off];
+      st1 = a.delta[(int64_t)bh * a.R + tile * BM + (int)(threadIdx.x & (BM - 1))];
+      st2 = pos0 + lim_off;
+      return;
+    }
     lq.load(a.D, [&](int n) {
       int pos, h;
       attn_row(a, min(tile * BM + n, a.R - 1), &pos, &h);
@@ -97,7 +132,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void k
     const int r = min(tile * BM + (int)(threadIdx.x & (BM - 1)), a.R - 1);
     int pos, h;
     attn_row(a, r, &pos, &h);
-    st0 = a.lse[((int64_t)b * a.Hkv * a.grp + hk * a.grp + h) * a.Nq + pos];
+    st0 = lsep[(int64_t)h * a.Nq + pos];
     st1 = a.delta[(int64_t)bh * a.R + r];
     st2 = pos + a.off;
   };
@@ -322,6 +357,10 @@ int attn_shape(const tts_attention_shape* s, AttnArgs* a, int* BH) {
   a->causal = s->causal != 0;
   a->off = (int)(s->keys - s->queries);
   a->scale = (float)s->scale;
+  const int64_t far = (int64_t)1 << 31, e = (int64_t)elem_size((int)s->dtype);
+  a->even_rows = 32 % grp == 0;
+  for (const int64_t* x : {s->q, s->dout})
+    if (x[1] < 0 || x[1] >= far || ((grp - 1) * x[1] + 64 * x[2] + 128) * e >= far) a->even_rows = 0;
   *BH = (int)(s->batch * s->kv_heads);
   return TTS_OK;
 }

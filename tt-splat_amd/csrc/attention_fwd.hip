@@ -86,12 +86,21 @@ void k_attn_fwd(AttnArgs a) {
   uint64_t live = 0;
   bool have = it.next(&t, &live);
   TileLoad<T, DP, BN, NT, ODD> lk, lv;
+  if constexpr (!ODD) {
+    lk.plan(a.D, [&](int n) { return n * a.sk.n; });
+    lv.plan(a.D, [&](int n) { return n * a.sv.n; });
+  }
   auto fetch = [&](int tile) {
     const int last = a.Nk - 1 - tile * BN;
     const T* k0 = kp + (int64_t)tile * BN * a.sk.n;
     const T* v0 = vp + (int64_t)tile * BN * a.sv.n;
-    lk.load_rows(a.D, k0, a.sk.n, last);
-    lv.load_rows(a.D, v0, a.sv.n, last);
+    if (!ODD && last >= BN - 1) {
+      lk.load_planned(k0);
+      lv.load_planned(v0);
+    } else {
+      lk.load_rows(a.D, k0, a.sk.n, last);
+      lv.load_rows(a.D, v0, a.sv.n, last);
+    }
   };
   auto put = [&](int buf, uint64_t bits) {
     lk.store(tk + buf * kTile, bits, a.D);
