@@ -18,6 +18,9 @@
 //           the whole device in the chunk pass, and no row walks more than 128 tokens, 128 chunks
 //           and tokens / 4096 spans.
 // Sums are held in 32 bits and rounded once.
+//
+// Bound: memory at a million tokens of 128 bf16 values (forward 76 us; gradient 209: sort 69, chunks 26,
+// rows 109), launches at 100 000 of 32 fp32 values (forward 6 us; gradient 39 in nine launches).
 
 #include "elem.h"
 
@@ -27,7 +30,7 @@ constexpr int kEmbBlock = 256;
 constexpr int kEmbWaves = kEmbBlock / 64;
 constexpr int kSmallPer = 16, kSmallTokens = kSmallPer * kEmbBlock;   // one block sorts up to 4096 tokens
 // Tokens a thread and a block of a pass over more: 1024 a block fill the card from 260 000 tokens on
-// (4096 a block: scatter of 100 000 tokens 15.4 -> TODO us, of a million 28.0 -> TODO).
+// (4096 a block: scatter of 100 000 tokens 15.4 -> 6.1 us, of a million 28.0 -> 20.8).
 constexpr int kPassPer = 4, kPassTokens = kPassPer * kEmbBlock;
 constexpr int kMaxDigitBits = 11;
 constexpr int kMaxBins = 1 << kMaxDigitBits;

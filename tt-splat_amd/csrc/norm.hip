@@ -14,6 +14,9 @@
 // dw and db: each block walks its share of the rows with the columns' sums in registers, joins its
 // waves in LDS in wave order and writes one row of partials; k_ln_join adds the blocks in order.
 // No atomics: the same inputs give the same bits.
+//
+// Measured: 1M x 64 bf16 forward 44 us (6.0 TB/s of its 0.26 GB, part of it still in the caches), backward
+// 75 + 6; 8040 x 1003 fp16 12 and 15 + 4.
 
 #include "elem.h"
 

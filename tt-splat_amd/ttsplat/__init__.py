@@ -17,6 +17,11 @@ Entry points mirror the reference's:
   ttsplat.model    GaussianModel in the [G,14] layout  (spike/model.py, resident_traced.py:91)
   ttsplat.scenes   the seeded benchmark configurations
   ttsplat.kernels  typed wrappers over every C entry point
+and, without a counterpart there, what a scene with several looks is trained with:
+  ttsplat.embedding   embedding: codes of gaussians and tokens, gradient by sorted tokens
+  ttsplat.norm        layer_norm
+  ttsplat.attention   attention: shared key heads, key masks, causal; recomputing backward
+  ttsplat.appearance  Appearance, fit_appearance, cell_codes: the three together
 """
 from . import camera, kernels, model, scenes  # noqa: F401
 
