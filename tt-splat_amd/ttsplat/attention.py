@@ -7,6 +7,7 @@ behind; the backward recomputes the probabilities.  Types fp32, fp16 and bf16; t
 sums are fp32.  Results are the same bits every time.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import kernels
 
@@ -32,6 +33,7 @@ class _Attention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, mask, out, rest, lse = ctx.saved_tensors
         causal, scale = ctx.meta

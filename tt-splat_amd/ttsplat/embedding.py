@@ -6,6 +6,7 @@ tokens by id and sums each row's tokens in token order in fp32: it is dense ([V,
 table) and the same bits every time.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import kernels
 
@@ -18,6 +19,7 @@ class _Embedding(torch.autograd.Function):
         return kernels.embedding_fwd(table, ids, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
         V, scale = ctx.meta

@@ -5,6 +5,7 @@ fp32, fp16 or bf16, weights of the same type or fp32; statistics and sums are fp
 gradients of weight and bias are summed over the rows in a fixed order.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import kernels
 
@@ -29,6 +30,7 @@ class _LayerNorm(torch.autograd.Function):
         return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         nx, nw, nb, _ = ctx.needs_input_grad
