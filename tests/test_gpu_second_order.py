@@ -29,5 +29,7 @@ def test_second_derivative_refused(name):
     # the square of the leaf has a second derivative of its own
     (g,) = torch.autograd.grad(run().square().sum() + leaf.square().sum(), leaf, create_graph=True)
     assert torch.equal(g, plain + 2 * leaf)
-    with pytest.raises(RuntimeError, match="once_differentiable"):
-        torch.autograd.grad(g.sum(), leaf)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(g.sum(), leaf, retain_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        g.sum().backward()

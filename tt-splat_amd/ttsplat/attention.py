@@ -7,9 +7,9 @@ behind; the backward recomputes the probabilities.  Types fp32, fp16 and bf16; t
 sums are fp32.  Results are the same bits every time.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels
+from .once import once
 
 F32 = torch.float32
 
@@ -33,14 +33,13 @@ class _Attention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
         q, k, v, mask, out, rest, lse = ctx.saved_tensors
         causal, scale = ctx.meta
         nq, nk, nv, _, _, _ = ctx.needs_input_grad
         grads = kernels._attention_bwd(q, k, v, mask, causal, scale, out, rest, lse,
                                        _last_contiguous(dout), nq, nk, nv)
-        return (*grads, None, None, None)
+        return (*once(grads, (q, k, v, dout)), None, None, None)
 
 
 def attention(q, k, v, key_mask=None, causal=False, scale=None):

@@ -6,9 +6,9 @@ tokens by id and sums each row's tokens in token order in fp32: it is dense ([V,
 table) and the same bits every time.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels
+from .once import once
 
 
 class _Embedding(torch.autograd.Function):
@@ -19,11 +19,11 @@ class _Embedding(torch.autograd.Function):
         return kernels.embedding_fwd(table, ids, scale)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
         V, scale = ctx.meta
-        return kernels._embedding_bwd(dout.contiguous(), ids, V, scale), None, None
+        dtable = kernels._embedding_bwd(dout.contiguous(), ids, V, scale)
+        return (*once((dtable,), (dout,)), None, None)
 
 
 def embedding(table, ids, scale=1.0):

@@ -5,9 +5,9 @@ fp32, fp16 or bf16, weights of the same type or fp32; statistics and sums are fp
 gradients of weight and bias are summed over the rows in a fixed order.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels
+from .once import once
 
 F32 = torch.float32
 
@@ -30,13 +30,13 @@ class _LayerNorm(torch.autograd.Function):
         return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         nx, nw, nb, _ = ctx.needs_input_grad
         dx, dw, db = kernels._layer_norm_bwd(_rows(x), weight, _rows(dy), stats, nx, nw, nb,
                                              ctx.w_dtype)
-        return (dx if dx is None or x.dim() == 2 else dx.view(x.shape)), dw, db, None
+        dx = dx if dx is None or x.dim() == 2 else dx.view(x.shape)
+        return (*once((dx, dw, db), (x, weight, dy)), None)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
