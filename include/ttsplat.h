@@ -660,7 +660,7 @@ typedef struct tts_attention_shape {
   int64_t dtype;        /* TTS_F32, TTS_F16 or TTS_BF16, of every tensor */
   int64_t mask_stride;  /* bytes between the batches of key_mask */
   int64_t q[3], k[3], v[3], o[3], dout[3], dq[3], dk[3], dv[3];
-  double scale;         /* positive; scores are scale * q . k */
+  double scale;         /* in [1e-30, 1e30]; scores are scale * q . k */
 } tts_attention_shape;
 
 /* Workspace of the forward (0 unless the keys are split) or the backward. */

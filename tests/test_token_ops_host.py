@@ -103,3 +103,13 @@ def test_wrappers_refuse_cpu_tensors():
                 lambda: embedding(x[0, 0], torch.zeros(3, dtype=torch.int64))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-39, 9e-31, 2e30])
+def test_attention_refuses_scales_past_fp32(lib, p, scale):
+    """1e-46 is 0 in fp32, the inverse of 1e-39 infinite: either gives NaN beside a hidden key."""
+    s = shape(scale=scale)
+    assert lib.tts_attention_fwd(s, p, p, p, None, p, None, None, None, 0, None) == EINVAL
+    assert lib.tts_attention_bwd(s, p, p, p, None, p, None, p, p, p, p, p, p, 1 << 40, None) == EINVAL
+    assert lib.tts_attention_workspace_bytes(shape(scale=1e-30), 1) > 0
+    assert lib.tts_attention_workspace_bytes(shape(scale=1e30), 1) > 0

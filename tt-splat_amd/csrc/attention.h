@@ -481,6 +481,9 @@ inline int launch_lds(K kernel, LdsLimit& lim, int blocks, int threads, size_t l
 }
 
 constexpr int kAttnMaxSplit = 64;
+// Scales whose inverse, and product with the log-sum-exp, stay normal fp32 numbers: a smaller one
+// would round to 0, which times a hidden key's -inf is NaN, or give an infinite inverse.
+constexpr double kAttnMinScale = 1.0e-30, kAttnMaxScale = 1.0e30;
 
 // Parts of `tiles` steps of the long axis for `waves` waves of work: as many as bring them nearest to
 // `fill`, each of `least` steps or more.

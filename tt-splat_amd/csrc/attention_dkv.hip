@@ -335,7 +335,7 @@ size_t attn_bwd_layout(AttnArgs& a, int64_t BH, const AttnPlan& p, char* base) {
 // Checks a shape's numbers and sets what both directions take from it.
 int attn_shape(const tts_attention_shape* s, AttnArgs* a, int* BH) {
   if (s->batch < 0 || s->kv_heads < 1 || s->heads < 1 || s->queries < 0 || s->keys < 0 ||
-      !(s->scale > 0.0) || !(s->scale < 3.0e38))
+      !(s->scale >= kAttnMinScale) || !(s->scale <= kAttnMaxScale))
     return TTS_EINVAL;
   if (s->head_dim < 1 || s->head_dim > 128 || s->heads % s->kv_heads) return TTS_EHEADS;
   if (s->dtype < 0 || s->dtype > 2) return TTS_EDTYPE;

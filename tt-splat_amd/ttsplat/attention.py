@@ -45,9 +45,9 @@ class _Attention(torch.autograd.Function):
 def attention(q, k, v, key_mask=None, causal=False, scale=None):
     """softmax(scale q k^T) v.  q [B, Hq, Nq, D], k and v [B, Hkv, Nk, D]: query head h reads key
     head h / (Hq / Hkv); any strides ([B, N, H, D] memory as a transposed view needs no copy), D up
-    to 128, scale 1/sqrt(D) unless given.  key_mask [B, Nk] bool or uint8: False hides a key (a
-    gaussian out of view, padding), whatever its k and v hold.  causal: row i sees keys up to
-    i + Nk - Nq.  A row that sees no key gives zeros and no gradient."""
+    to 128, scale 1/sqrt(D) unless given (1e-30 to 1e30).  key_mask [B, Nk] bool or uint8: False
+    hides a key (a gaussian out of view, padding), whatever its k and v hold.  causal: row i sees
+    keys up to i + Nk - Nq.  A row that sees no key gives zeros and no gradient."""
     q, k, v = _last_contiguous(q), _last_contiguous(k), _last_contiguous(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         mask, scale = kernels._attn_check(q, k, v, key_mask, scale, None)

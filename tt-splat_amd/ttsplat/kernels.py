@@ -1226,8 +1226,8 @@ def _attn_check(q, k, v, key_mask, scale, out):
     if not 1 <= D <= 128:
         raise ValueError(f"head size must be in [1, 128], got {D}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"scale must be in [1e-30, 1e30], got {scale}")
     if out is not None:
         _attn_tensor(out, "out", q.shape, dt, dev)
     if key_mask is not None:
