@@ -396,8 +396,10 @@ __device__ __forceinline__ void store_column(T* row, int D, int db, const Acc& x
 }
 
 // Joins the parts of split rows, in order: G groups of L lanes a row, each of which takes every G-th
-// part; the groups' sums are joined in a tree.  x: four columns' sum from column c on.  lse (softmax
-// parts): the parts' log-sum-exps weigh them, *m and *l are the maximum and the weights' sum.
+// part; the groups' sums are joined in a tree, and where a block takes one row (BLOCK: L G = 256) its
+// waves' by way of LDS.  x: four columns' sum from column c on, in group 0.  lse (softmax parts): the
+// parts' log-sum-exps weigh them, join_max is their maximum, *l the weights' sum.
+constexpr int kJoinLanes = 32;   // 128 columns
 struct JoinTeam {
   int lig, g, L, G;
   int64_t row;
@@ -405,14 +407,21 @@ struct JoinTeam {
       : lig(threadIdx.x & (L_ - 1)), g(threadIdx.x / L_ & (G_ - 1)), L(L_), G(G_),
         row((int64_t)blockIdx.x * (256 / (L_ * G_)) + threadIdx.x / (L_ * G_)) {}
 };
+template <bool BLOCK>
 __device__ __forceinline__ float join_max(const JoinTeam& t, const float* lse, int64_t rows,
                                           int nsplit) {
   float m = -INFINITY;
   for (int s = t.g * t.L + t.lig; s < nsplit; s += t.L * t.G) m = fmaxf(m, lse[s * rows + t.row]);
-  for (int o = 1; o < t.L * t.G; o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
+  for (int o = 1; o < (BLOCK ? 64 : t.L * t.G); o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if constexpr (BLOCK) {
+    __shared__ float red[4];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
   return m;
 }
-template <bool SOFT>
+template <bool SOFT, bool BLOCK = false>
 __device__ __forceinline__ void join_parts(const JoinTeam& t, const float* part, const float* lse,
                                            int64_t rows, int nsplit, int D4, int c, float m,
                                            float* l, float (&x)[4]) {
@@ -429,10 +438,28 @@ __device__ __forceinline__ void join_parts(const JoinTeam& t, const float* part,
     x[2] += w * v.z;
     x[3] += w * v.w;
   }
-  for (int o = t.L; o < t.L * t.G; o *= 2) {
+  for (int o = t.L; o < (BLOCK ? 64 : t.L * t.G); o *= 2) {
     *l += __shfl_xor(*l, o, 64);
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] += __shfl_xor(x[j], o, 64);
+  }
+  if constexpr (BLOCK) {   // L lanes cover the columns: once a row
+    __shared__ float red[5][4][kJoinLanes];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (lane < t.L) {
+      red[4][wave][lane] = *l;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) red[j][wave][lane] = x[j];
+    }
+    __syncthreads();
+    if (t.g == 0) {
+      auto sum = [&](int j) {
+        return (red[j][0][lane] + red[j][1][lane]) + (red[j][2][lane] + red[j][3][lane]);
+      };
+      *l = sum(4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = sum(j);
+    }
   }
 }
 

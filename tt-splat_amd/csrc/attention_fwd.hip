@@ -242,8 +242,8 @@ void k_attn_fwd(AttnArgs a) {
   }
 }
 
-// Joins the parts of split rows.
-template <typename T>
+// Joins the parts of split rows; BLOCK: a block a row.
+template <typename T, bool BLOCK>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int BH, int L, int G) {
   const JoinTeam t(L, G);
   const int64_t rows = (int64_t)BH * a.R;
@@ -253,13 +253,13 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int BH, int L, in
   int pos, h;
   attn_row(a, row, &pos, &h);
   const int hq = hk * a.grp + h;
-  const float mx = join_max(t, a.part2, rows, a.nsplit), m = mx == -INFINITY ? 0.0f : mx;
+  const float mx = join_max<BLOCK>(t, a.part2, rows, a.nsplit), m = mx == -INFINITY ? 0.0f : mx;
   T* op = static_cast<T*>(a.out) + b * a.so.b + hq * a.so.h + (int64_t)pos * a.so.n;
   float l = 0.0f;
   for (int c0 = 0; c0 < a.D; c0 += L * 4) {
     const int c = c0 + t.lig * 4;
     float x[4];
-    join_parts<true>(t, a.part, a.part2, rows, a.nsplit, a.D4, c, m, &l, x);
+    join_parts<true, BLOCK>(t, a.part, a.part2, rows, a.nsplit, a.D4, c, m, &l, x);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (t.g == 0) {
 #pragma unroll
@@ -297,8 +297,16 @@ int attn_launch_fwd(const AttnArgs& a0, int BH, int dtype, const AttnPlan& p, hi
     });
     if (e || p.fs == 1) return e;
     int L, G;
-    join_shape((int64_t)BH * a.R, a.D, a.nsplit, &L, &G);
-    k_attn_join<T><<<join_blocks((int64_t)BH * a.R, L, G), 256, 0, stream>>>(a, BH, L, G);
+    const int64_t rows = (int64_t)BH * a.R;
+    join_shape(rows, a.D, a.nsplit, &L, &G);
+    // Up to a row a CU, such as single tokens': a block each, where that leaves each group a part or more
+    // (64 rows of 64 parts: a waited-for call 44.5 -> 40.7 us, a call among others 20.1 -> 19.6).
+    if (rows <= 256 && a.nsplit * L >= 256) {
+      G = 256 / L;
+      k_attn_join<T, true><<<(int)rows, 256, 0, stream>>>(a, BH, L, G);
+    } else {
+      k_attn_join<T, false><<<join_blocks(rows, L, G), 256, 0, stream>>>(a, BH, L, G);
+    }
     return launch_status();
   });
 }
