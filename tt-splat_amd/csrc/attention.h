@@ -357,6 +357,22 @@ __device__ __forceinline__ Frag<T> acc_frag(const Acc& s, int c) {
   return f;
 }
 
+// What that rounding left out, as an operand of a second product.
+template <typename T>
+__device__ __forceinline__ Frag<T> acc_rest(const Acc& s, int c, Frag<T> f) {
+  Frag<T> r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = (T)(s[8 * c + j] - (float)f[j]);
+  return r;
+}
+// Half types, odd heads of up to 32 values: the forward's P and dQ's dS go into their products in two parts.
+// A row's dS sum to zero, and the fewer values a head has, the more alike are the keys that a row
+// weighs most: the terms dS K cancel, while an error of D, which P's rounding in O brings, is multiplied
+// by all of sum P K (one value, two rows over 4099 keys, fp16: dQ 1.7 u off in the mean, 1.2 u with dS in
+// two parts alone; u = 2^-11).
+template <typename T, int DP, bool ODD>
+constexpr bool kTwoParts = sizeof(T) == 2 && ODD && DP == 32;
+
 // Four consecutive values of a row, n of them within it.
 template <typename T>
 __device__ __forceinline__ void store4(T* p, int n, float x0, float x1, float x2, float x3) {

@@ -6,7 +6,8 @@
 // this kernel and the keys' one computes S and dP twice (7 products in place of 5), and needs no
 // atomics, no partial dQ for each block of keys, and gives the same bits every time.
 //
-// dS is rounded to the operands' type for its product (half types); everything else is fp32.
+// dS is rounded to the operands' type for its product (half types); everything else is fp32.  (Odd heads of up
+// to 32 values: kTwoParts.)
 //
 // Measured: 8040 x 8040, 16 heads of 128 bf16, 870 us (910 TFLOP/s); 2500 x 2500, 16 heads of 64: 66 us.
 // Tiles of 32 keys in place of 64: 906 -> 1018.
@@ -151,9 +152,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && (NW > 1 || DP <= 64) ? 2
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const Frag<T> ds = acc_frag<T>(s, c);
+        Frag<T> rest;
+        if constexpr (kTwoParts<T, DP, ODD>) rest = acc_rest(s, c, ds);
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-          dq[d] = mma(transpose_frag<T, DP>(sk, kb * 32 + c * 16, d * 32), ds, dq[d]);
+        for (int d = 0; d < DB; ++d) {
+          const Frag<T> f = transpose_frag<T, DP>(sk, kb * 32 + c * 16, d * 32);
+          dq[d] = mma(f, ds, dq[d]);
+          if constexpr (kTwoParts<T, DP, ODD>) dq[d] = mma(f, rest, dq[d]);
+        }
       }
     }
     if (more) put(buf ^ 1, ln);

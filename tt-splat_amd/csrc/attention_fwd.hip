@@ -6,7 +6,7 @@
 // the wave are joined once a tile (maximum) and once at the end (sum).
 //
 // Roundings: S, the softmax and O are fp32; P is rounded to the operands' type for its product with V
-// (half types), O once at the end.
+// (half types; odd heads of up to 32 values: kTwoParts), O once at the end.
 //
 // For a backward in half types the rounding's rest, O - (T)O, is stored beside O: D = rowsum(dO O) then
 // carries 16 bits of O, not 8 or 11 (without it dQ and dK of short key axes lose a quarter of a bit).
@@ -190,14 +190,20 @@ void k_attn_fwd(AttnArgs a) {
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        Frag<T> p[QB];
+        Frag<T> p[QB], rest[QB];
 #pragma unroll
-        for (int j = 0; j < QB; ++j) p[j] = acc_frag<T>(s[kb][j], c);
+        for (int j = 0; j < QB; ++j) {
+          p[j] = acc_frag<T>(s[kb][j], c);
+          if constexpr (kTwoParts<T, DP, ODD>) rest[j] = acc_rest(s[kb][j], c, p[j]);
+        }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           const Frag<T> f = transpose_frag<T, DP>(sv, kb * 32 + c * 16, d * 32);
 #pragma unroll
-          for (int j = 0; j < QB; ++j) o[j][d] = mma(f, p[j], o[j][d]);
+          for (int j = 0; j < QB; ++j) {
+            o[j][d] = mma(f, p[j], o[j][d]);
+            if constexpr (kTwoParts<T, DP, ODD>) o[j][d] = mma(f, rest[j], o[j][d]);
+          }
         }
       }
     }
