@@ -149,6 +149,13 @@ __global__ __launch_bounds__(kLnBlock) void k_ln_fwd_wide(const T* __restrict__ 
   }
 }
 
+// dy w, rounded: fused into g - mean g its rounding's rest would stay where they are equal (rows of one
+// column have dx = 0).
+__device__ __forceinline__ float ln_weighted(float dy, float w) {
+#pragma clang fp contract(off)
+  return dy * w;
+}
+
 // dx of the block's rows and its partial sums of dy xh and dy, part[block][2][cols].
 template <typename T, int L, int NV, int MODE>
 __global__ __launch_bounds__(kLnBlock) void k_ln_bwd(const T* __restrict__ x, int64_t xs,
@@ -187,7 +194,7 @@ __global__ __launch_bounds__(kLnBlock) void k_ln_bwd(const T* __restrict__ x, in
         v[j][i] = (v[j][i] - st.x) * st.y;   // past the row: g is zero there, so it adds nothing
         aw[j][i] += g[j][i] * v[j][i];
         ab[j][i] += g[j][i];
-        g[j][i] *= wt[j][i];
+        g[j][i] = ln_weighted(g[j][i], wt[j][i]);
         s1 += g[j][i];
         s2 += g[j][i] * v[j][i];
       }
@@ -262,7 +269,7 @@ __global__ __launch_bounds__(kLnBlock) void k_ln_bwd_wide(const T* __restrict__ 
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           v[i] = (v[i] - st.x) * st.y;
-          g[i] *= wt[i];
+          g[i] = ln_weighted(g[i], wt[i]);
           if (pass == 0) {
             s1 += g[i];
             s2 += g[i] * v[i];
