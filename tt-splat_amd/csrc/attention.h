@@ -369,7 +369,7 @@ __device__ __forceinline__ Frag<T> acc_rest(const Acc& s, int c, Frag<T> f) {
 // A row's dS sum to zero, and the fewer values a head has, the more alike are the keys that a row
 // weighs most: the terms dS K cancel, while an error of D, which P's rounding in O brings, is multiplied
 // by all of sum P K (one value, two rows over 4099 keys, fp16: dQ 1.7 u off in the mean, 1.2 u with dS in
-// two parts alone; u = 2^-11).
+// two parts alone; u = 2^-11).  Costs 12 % at 20 values, 2500 x 2500, 16 heads, bf16, gradients: 189 -> 211 us.
 template <typename T, int DP, bool ODD>
 constexpr bool kTwoParts = sizeof(T) == 2 && ODD && DP == 32;
 
